@@ -320,6 +320,38 @@ int vi_interp_band(int kind, uint64_t* out, int64_t out_off, int64_t flat_lo, in
                    int64_t aux_n, const uint8_t* seed_dev, const uint8_t* label_dev, int label_len,
                    void* stream);
 
+/* ---- the quantised model beside the prover -----------------------------------------
+ * No counterpart in the reference, whose callers bring integers that are already quantised (prover/loader.py:61-70) and
+ * multiply them as field elements (gl_matmul).  Element types of inputs and outputs: */
+enum { VI_F32 = 0, VI_F16 = 1, VI_BF16 = 2, VI_I32 = 3, VI_FIELD = 4 };
+
+/* Rows to int8 with one scale a row: x (m, k) of VI_F32 / VI_F16 / VI_BF16, rows x_stride elements apart;
+ * scale[r] = max_j |x_rj| / 127, q_rj = the whole number nearest to 127 x_rj / max_j |x_rj| (of the exact quotient, ties
+ * to even), in rows q_stride bytes apart.  A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN and
+ * q = 0. */
+int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t x_stride,
+                          int8_t* q, int64_t q_stride, float* scale, void* stream);
+
+/* S = A.B of int8 matrices, exact in 32 bits (k <= 131071).  A (m, k), rows lda bytes apart; B (k, n) with rows ldb bytes
+ * apart, or, with b_by_channel, stored (n, k) with the k values of a channel together and channels ldb bytes apart.
+ * out_type VI_F32 / VI_F16 / VI_BF16: C_ij = (S_ij * sa_i) * sb_j in fp32, rounded once to the type (sa (m), sb (n); NULL =
+ * ones); VI_I32: S; VI_FIELD: S mod p as uint64_t, negative sums as p - |S| (the same value vi_gl_matmul gives for the
+ * lifted operands); these two take no scales.  C rows ldc elements apart. */
+int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel,
+                   const float* sa, const float* sb, void* C, int out_type, int64_t ldc,
+                   int64_t m, int64_t k, int64_t n, void* stream);
+
+/* What each row of logits (rows x vocab, `stride` elements apart, VI_F32 / VI_F16 / VI_BF16) says about its token, with
+ * p = softmax(x / temperature): logprob[r] = log p[tokens[r]] (0 where the token is negative: no token at this position;
+ * NaN where it is vocab or more), entropy[r] = -sum p log p, and the `top` (0 .. 32) likeliest tokens in falling order, ties
+ * to the lowest index, with their log probabilities: top_logprob, top_token (rows x top).  Natural logarithms.  Entries of
+ * -inf are tokens that are not allowed; where fewer than `top` are left, the rest of the list is -1 with -inf.  A row of
+ * nothing but -inf has logprob -inf and entropy 0; one that holds a NaN or +inf has NaN in all its numbers and an empty
+ * list.  1e-6 <= temperature <= 1e6. */
+int vi_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
+                      const int64_t* tokens, int top, float temperature,
+                      float* logprob, float* entropy, float* top_logprob, int64_t* top_token, void* stream);
+
 /* ---- per-kernel timing ------------------------------------------------------------
  * CUDA events recorded around every launch on the launching stream while enabled (the
  * reference's nearest equivalent is its LIGERO_EPHASE event sums, prover/core.py:1139-1165).

@@ -1,0 +1,560 @@
+"""The quantised model's operators: int8 rows, int8 products, token log probabilities, against plain implementations in 64
+bits; what they refuse; a run of them together.  Tolerances are counted in roundings: half a step is 2^-24 of the value in
+fp32, 2^-11 in fp16, 2^-8 in bf16."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+P = (1 << 64) - (1 << 32) + 1
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from verinf_b200 import _lib
+    return _lib
+
+
+@pytest.fixture(scope="module")
+def i8():
+    from verinf_b200 import int8
+    return int8
+
+
+@pytest.fixture(scope="module")
+def lp():
+    from verinf_b200 import logprobs
+    return logprobs
+
+
+# ---- refusals of the C ABI, before any kernel runs (no GPU) -------------------------------------------------------
+def _err(lib):
+    return lib.LIB.vi_last_error().decode()
+
+
+def _buf():
+    b = (C.c_uint64 * 64)()
+    return b, C.cast(b, C.c_void_p).value
+
+
+def test_quantize_refusals_without_gpu(lib):
+    L = lib.LIB
+    keep, p = _buf()
+    assert L.vi_int8_quantize_rows(p, 3, 1, 4, 4, p, 4, p, None) != 0 and "dtype" in _err(lib)
+    assert L.vi_int8_quantize_rows(p, 0, -1, 4, 4, p, 4, p, None) != 0 and "negative" in _err(lib)
+    assert L.vi_int8_quantize_rows(p, 0, 1 << 31, 4, 4, p, 4, p, None) != 0 and "rows" in _err(lib)
+    assert L.vi_int8_quantize_rows(p, 0, 2, 4, 3, p, 4, p, None) != 0 and "overlap" in _err(lib)
+    assert L.vi_int8_quantize_rows(p, 0, 2, 4, 4, p, 3, p, None) != 0 and "overlap" in _err(lib)
+    assert L.vi_int8_quantize_rows(p + 2, 0, 1, 4, 4, p, 4, p, None) != 0 and "aligned" in _err(lib)
+    assert L.vi_int8_quantize_rows(p, 0, 1, 4, 4, p, 4, None, None) != 0 and "scale" in _err(lib)
+    assert L.vi_int8_quantize_rows(None, 0, 1, 4, 4, p, 4, p, None) != 0 and "null" in _err(lib)
+    assert L.vi_int8_quantize_rows(None, 0, 0, 4, 4, None, 4, None, None) == 0
+
+
+def test_matmul_refusals_without_gpu(lib):
+    L = lib.LIB
+    keep, p = _buf()
+
+    def call(A=p, lda=4, B=p, ldb=4, nk=0, sa=None, sb=None, Cp=p, out=3, ldc=4, m=2, k=4, n=4):
+        return L.vi_int8_matmul(A, lda, B, ldb, nk, sa, sb, Cp, out, ldc, m, k, n, None)
+    assert call(m=-1) != 0 and "negative" in _err(lib)
+    assert call(out=5) != 0 and "output type" in _err(lib)
+    assert call(out=-1) != 0 and "output type" in _err(lib)
+    assert call(k=131072) != 0 and "131071" in _err(lib)
+    assert call(out=3, sa=p) != 0 and "no scales" in _err(lib)
+    assert call(out=4, sb=p) != 0 and "no scales" in _err(lib)
+    assert call(Cp=None) != 0 and "output" in _err(lib)
+    assert call(Cp=p + 2) != 0 and "misaligned output" in _err(lib)
+    assert call(ldc=3) != 0 and "overlap" in _err(lib)
+    assert call(A=None) != 0 and "null input" in _err(lib)
+    assert call(out=0, sa=p + 1) != 0 and "scales" in _err(lib)
+    assert call(m=0, A=None, Cp=None) == 0
+    assert call(n=0, A=None, Cp=None) == 0
+
+
+def test_logprobs_refusals_without_gpu(lib):
+    L = lib.LIB
+    keep, p = _buf()
+
+    def call(x=p, dtype=0, rows=1, vocab=4, stride=4, tok=p, top=0, t=1.0, a=p, b=p, tl=p, tt=p):
+        return L.vi_token_logprobs(x, dtype, rows, vocab, stride, tok, top, t, a, b, tl, tt, None)
+    assert call(dtype=3) != 0 and "dtype" in _err(lib)
+    assert call(rows=-1) != 0
+    assert call(vocab=0) != 0 and "vocab" in _err(lib)
+    assert call(vocab=1 << 31) != 0 and "limited" in _err(lib)
+    assert call(top=33) != 0 and "top" in _err(lib)
+    assert call(top=-1) != 0 and "top" in _err(lib)
+    for t in (0.0, -1.0, float("nan"), float("inf")):
+        assert call(t=t) != 0 and "temperature" in _err(lib)
+    assert call(x=None) != 0 and "null" in _err(lib)
+    assert call(top=1, tl=None) != 0 and "null" in _err(lib)
+    assert call(x=p + 2) != 0 and "aligned" in _err(lib)
+    assert call(tok=p + 4) != 0 and "misaligned" in _err(lib)
+    assert call(rows=2, stride=-4) != 0 and "stride" in _err(lib)
+    assert call(rows=0, x=None, tok=None) == 0
+
+
+def test_python_refusals_without_gpu(i8, lp):
+    with pytest.raises(RuntimeError, match="CUDA"):
+        i8.int8_quantize_rows(torch.zeros(2, 3))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        i8.int8_matmul(torch.zeros(2, 3, dtype=torch.int8), torch.zeros(3, 2, dtype=torch.int8))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        lp.token_logprobs(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64))
+
+
+# ---- rows to int8 --------------------------------------------------------------------------------------------------
+def _quantize_64(x):
+    """In 64 bits the quotient of 31-bit by 24-bit numbers never rounds onto a border that it is not on: it differs from a
+    half-integer by at least 2^-33 of itself."""
+    x = x.detach().cpu().double()
+    big = x.abs().amax(1, keepdim=True) if x.size(1) else torch.zeros(x.size(0), 1, dtype=torch.float64)
+    bad = ~torch.isfinite(x).all(1)
+    safe = torch.where((big > 0) & torch.isfinite(big), big, 1.0)
+    q = torch.where(bad[:, None], 0.0, torch.nan_to_num(127 * x / safe, 0, 0, 0)).round().to(torch.int8)
+    scale = big[:, 0].float() / np.float32(127)                     # one division in fp32
+    return q, torch.where(bad, float("nan"), scale)
+
+
+def _check_quantize(i8, x, **kw):
+    q, s = i8.int8_quantize_rows(x, **kw)
+    wq, ws = _quantize_64(x)
+    assert torch.equal(q.cpu(), wq)
+    assert torch.equal(torch.nan_to_num(s.cpu(), -1), torch.nan_to_num(ws, -1))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 7), (3, 8), (2, 129), (5, 1000), (1, 4096), (33, 5003), (2, 16384), (2, 40001), (1000, 96)])
+def test_quantize_sizes(i8, dtype, m, k):
+    g = torch.Generator().manual_seed(m * 7919 + k)
+    x = (torch.randn(m, k, generator=g) * torch.exp(3 * torch.randn(m, 1, generator=g))).to(dtype).cuda()
+    _check_quantize(i8, x)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantize_borders(i8, dtype):
+    """Rows whose quotients fall on borders exactly, or next to them: maxima 127 and 254 with halves, neighbours of halves."""
+    halves = torch.arange(-127, 127).double() + 0.5
+    rows = [torch.cat([halves, torch.tensor([127.0])]), torch.cat([2 * halves, torch.tensor([-254.0])]),
+            torch.cat([halves * 4, torch.tensor([127.0 * 4])])]
+    near = [torch.nextafter(halves.float(), torch.full_like(halves.float(), s)).double() for s in (-1e9, 1e9)]
+    rows += [torch.cat([n, torch.tensor([127.0])]) for n in near]
+    x = torch.stack(rows).to(dtype)
+    _check_quantize(i8, x.cuda())
+    odd = torch.stack([torch.cat([halves * f, torch.tensor([127.0 * f])]) for f in (1 / 3, 0.7, 1.1, 97.3)]).to(dtype)
+    _check_quantize(i8, odd.cuda())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantize_extremes(i8, dtype):
+    """The type's largest, smallest and subnormal values, rows of zeros, rows with NaN and infinities."""
+    f = torch.finfo(dtype)
+    tiny = f.smallest_normal * f.eps                                # the least subnormal value
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(8, 300, generator=g).double().clamp(-1, 1)
+    base[:, 0] = 1
+    x = torch.zeros(12, 300, dtype=dtype)
+    x[0] = (base[0] * f.max).to(dtype)
+    x[1] = (base[1] * f.smallest_normal).to(dtype)
+    x[2] = (base[2] * tiny * 5).to(dtype)
+    x[3, 17] = tiny
+    x[4, 5] = -f.max
+    x[4, 6] = tiny
+    x[6] = base[3].to(dtype); x[6, 299] = float("nan")
+    x[7] = base[4].to(dtype); x[7, 0] = float("inf")
+    x[8] = base[5].to(dtype); x[8, 131] = -float("inf")
+    x[9] = (base[6] * f.smallest_normal * 64).to(dtype)
+    x[10] = -0.0
+    x[11] = (base[7] * f.smallest_normal * 3).to(dtype)
+    _check_quantize(i8, x.cuda())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("offset,pitch", [(0, 1040), (0, 1033), (1, 1040), (3, 1029), (8, 1040)])
+def test_quantize_strides_and_out(i8, dtype, offset, pitch):
+    g = torch.Generator().manual_seed(offset + pitch)
+    k = 1003
+    buf = torch.randn(9, pitch + 16, generator=g).to(dtype).cuda()
+    x = buf[:, offset:offset + k]
+    _check_quantize(i8, x)
+    room = torch.full((9, pitch), 77, dtype=torch.int8, device="cuda")
+    scale = torch.empty(9, device="cuda")
+    q, s = i8.int8_quantize_rows(x, out=(room[:, 5:5 + k], scale))
+    wq, ws = _quantize_64(x)
+    assert torch.equal(room[:, 5:5 + k].cpu(), wq) and torch.equal(scale.cpu(), ws)
+    assert (room[:, :5] == 77).all() and (room[:, 5 + k:] == 77).all()
+    _check_quantize(i8, x[:1].expand(4, k))
+
+
+@gpu
+def test_quantize_empty_and_refusals(i8):
+    q, s = i8.int8_quantize_rows(torch.empty(0, 5, device="cuda"))
+    assert q.shape == (0, 5) and s.shape == (0,)
+    q, s = i8.int8_quantize_rows(torch.empty(3, 0, device="cuda"))
+    assert q.shape == (3, 0) and (s == 0).all()
+    x = torch.zeros(4, 6, device="cuda")
+    q, s = torch.empty(4, 6, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
+    for bad, words in [((x.double(),), "dtype"), ((x[0],), "2-D"), ((x.t(),), "lie together")]:
+        with pytest.raises(RuntimeError, match=words):
+            i8.int8_quantize_rows(*bad)
+    for out, words in [((q[:3], s), "shape"), ((q.to(torch.int32), s), "dtype"), ((q[:1].expand(4, 6), s), "overlap"),
+                       ((q, s[:3]), "scales"), ((q, s.double()), "scales"), ((q, s.cpu()), "scales"), ((q.cpu(), s), "CUDA"),
+                       ((torch.empty(6, 4, dtype=torch.int8, device="cuda").t(), s), "lie together")]:
+        with pytest.raises(RuntimeError, match=words):
+            i8.int8_quantize_rows(x, out=out)
+
+
+# ---- product --------------------------------------------------------------------------------------------------------
+def _sums_64(A, B):
+    return (A.cpu().double() @ B.cpu().double()).to(torch.int64)        # |sum| < 2^31: whole in 64-bit floats
+
+
+def _field(S):
+    return np.where(S.numpy() < 0, S.numpy() + np.int64(P - (1 << 64)), S.numpy())
+
+
+def _rand8(g, *shape):
+    return torch.randint(-128, 128, shape, generator=g, dtype=torch.int8)
+
+
+def _weight(g, k, n, layout, pad):
+    """(k, n) int8 on the GPU: row-major ("kn") or by channel ("nk"), `pad` bytes behind each row or channel."""
+    r, c = (k, n) if layout == "kn" else (n, k)
+    buf = _rand8(g, r, c + pad).cuda()[:, :c]
+    return buf if layout == "kn" else buf.t()
+
+
+def _check_matmul(i8, A, B, dtypes=None, g=None, out_pad=0):
+    m, n = A.size(0), B.size(1)
+    S = _sums_64(A, B)
+    for dtype in dtypes or [torch.int32, torch.uint64] + FLOATS:
+        out = None
+        if out_pad:
+            room = torch.full((m, n + out_pad), 7, device="cuda").to(dtype) if dtype != torch.uint64 else \
+                torch.full((m, n + out_pad), 7, dtype=torch.int64, device="cuda").view(torch.uint64)
+            out = room[:, :n]
+        if dtype == torch.int32:
+            assert torch.equal(i8.int8_matmul(A, B, dtype=dtype, out=out).cpu().to(torch.int64), S)
+        elif dtype == torch.uint64:
+            got = i8.int8_matmul(A, B, dtype=dtype, out=out).view(torch.int64).cpu().numpy()
+            assert np.array_equal(got, _field(S))
+        else:
+            sa = torch.rand(m, generator=g) * 0.05 + 1e-3
+            sb = torch.rand(n, generator=g) * 0.02 + 1e-4
+            got = i8.int8_matmul(A, B, sa.cuda(), sb.cuda(), dtype=dtype, out=out).cpu().double()
+            want = S.double() * sa.double()[:, None] * sb.double()
+            # roundings: the sum to fp32, two products, the output type (fp32: the second product already is it)
+            tol = want.abs() * (3 * HALF[torch.float32] + (HALF[dtype] if dtype != torch.float32 else 0)) * 1.001
+            tol = tol + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+            big = want.abs() > torch.finfo(dtype).max
+            assert ((got - want).abs() <= tol)[~big].all() and torch.isinf(got[big & (want.abs() > 2 * torch.finfo(dtype).max)]).all()
+        if out_pad:
+            assert (room.view(torch.int64 if dtype == torch.uint64 else dtype)[:, n:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 16, 8), (2, 3, 5), (7, 33, 9), (1, 4096, 512), (3, 1000, 130), (16, 128, 128),
+                                   (17, 257, 129), (31, 515, 1001), (64, 1024, 256), (65, 48, 300), (128, 384, 640), (129, 1001, 515),
+                                   (255, 64, 31), (300, 2048, 384), (513, 640, 272)])
+def test_matmul_sizes(i8, layout, m, k, n):
+    g = torch.Generator().manual_seed(m + 31 * k + 101 * n)
+    _check_matmul(i8, _rand8(g, m, k).cuda(), _weight(g, k, n, layout, 0), g=g)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("m", [1, 5, 40, 200])
+@pytest.mark.parametrize("pad,a_pad,offset", [(0, 0, 1), (16, 32, 0), (5, 3, 0), (11, 0, 7), (0, 9, 0)])
+def test_matmul_strides(i8, layout, m, pad, a_pad, offset):
+    g = torch.Generator().manual_seed(m + pad + a_pad + offset)
+    k, n = 272, 336
+    A = _rand8(g, m, k + a_pad + offset).cuda()[:, offset:offset + k]
+    B = _weight(g, k + offset, n + offset, layout, pad)[offset:, offset:]
+    _check_matmul(i8, A, B, [torch.int32, torch.bfloat16], g)
+    _check_matmul(i8, A, B, g=g, out_pad=3)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 33, 300])
+def test_matmul_extreme_sums(i8, m):
+    """The largest sums: every product 2^14 at the longest k, either sign."""
+    k, n = 131071, 24
+    A = torch.full((m, k), -128, dtype=torch.int8, device="cuda")
+    B = torch.full((n, k), -128, dtype=torch.int8, device="cuda")
+    B[1::2] = 127
+    got = i8.int8_matmul(A, B.t())
+    assert (got[:, 0::2] == 16384 * k).all() and (got[:, 1::2] == -16256 * k).all()
+    got = i8.int8_matmul(A, B.t(), dtype=torch.uint64).view(torch.int64)
+    assert (got[:, 0::2] == 16384 * k).all() and (got[:, 1::2] == P - (1 << 64) - 16256 * k).all()
+
+
+@gpu
+def test_matmul_scales(i8):
+    """Missing scales are ones, an infinite or NaN scale reaches its row or column only, results beyond fp16 are infinite."""
+    g = torch.Generator().manual_seed(3)
+    A, B = _rand8(g, 20, 64).cuda(), _weight(g, 64, 40, "nk", 0)
+    S = _sums_64(A, B)
+    assert torch.equal(i8.int8_matmul(A, B, dtype=torch.float32).cpu(), S.float())
+    sa = torch.ones(20, device="cuda"); sa[4] = float("nan")
+    y = i8.int8_matmul(A, B, sa, dtype=torch.float32).cpu()
+    assert torch.isnan(y[4]).all() and torch.equal(y[[3, 5]], S[[3, 5]].float())
+    sb = torch.full((40,), 2.0, device="cuda"); sb[7] = 1e30
+    y = i8.int8_matmul(A, B, None, sb, dtype=torch.float16).cpu()
+    assert torch.isinf(y[:, 7][S[:, 7] != 0]).all() and torch.equal(y[:, 6], (2 * S[:, 6]).half())
+
+
+@gpu
+def test_matmul_empty_and_refusals(i8):
+    z = lambda *s: torch.zeros(s, dtype=torch.int8, device="cuda")
+    assert i8.int8_matmul(z(0, 4), z(4, 3)).shape == (0, 3)
+    assert i8.int8_matmul(z(2, 4), z(4, 0)).shape == (2, 0)
+    assert (i8.int8_matmul(z(2, 0), z(0, 3)) == 0).all()
+    assert (i8.int8_matmul(z(2, 0), z(0, 3), torch.full((2,), 3.0, device="cuda"), dtype=torch.bfloat16) == 0).all()
+    g = torch.Generator().manual_seed(1)
+    A = _rand8(g, 1, 40).cuda().expand(6, 40)                      # expanded operands
+    B = _rand8(g, 40, 1).cuda().expand(40, 24)
+    assert torch.equal(i8.int8_matmul(A, B).cpu().long(), _sums_64(A, B))
+    B = _rand8(g, 1, 24).cuda().expand(40, 24)
+    assert torch.equal(i8.int8_matmul(A, B).cpu().long(), _sums_64(A, B))
+    one = torch.ones
+    for args, kw, words in [((z(2, 3), z(4, 2)), {}, "inner dim"), ((z(2, 3).float(), z(3, 2)), {}, "dtype"), ((z(2, 3)[0], z(3, 2)), {}, "2-D"),
+                            ((z(2, 3), z(3, 2).cpu()), {}, "CUDA"), ((z(2, 3), z(3, 2)), dict(dtype=torch.float64), "dtype must be"),
+                            ((z(2, 3), z(3, 2), one(2, device="cuda")), {}, "no scales"),
+                            ((z(2, 3), z(3, 2), one(3, device="cuda")), dict(dtype=torch.float16), "scale_a"),
+                            ((z(2, 3), z(3, 2), one(2)), dict(dtype=torch.float16), "scale_a"),
+                            ((z(2, 3), z(3, 2), None, one(2, device="cuda").double()), dict(dtype=torch.float16), "scale_b"),
+                            ((z(3, 2).t(), z(3, 2)), {}, "lie together"), ((z(2, 3), z(6, 4)[::2, ::2]), {}, "lie together"),
+                            ((z(1, 131072), z(131072, 1)), {}, "131071"),
+                            ((z(2, 3), z(3, 2)), dict(out=torch.empty(2, 2, device="cuda")), "out"),
+                            ((z(2, 3), z(3, 2)), dict(out=torch.empty(2, 3, dtype=torch.int32, device="cuda")), "out must"),
+                            ((z(2, 3), z(3, 2)), dict(out=torch.empty(1, 2, dtype=torch.int32, device="cuda").expand(2, 2)), "overlap")]:
+        with pytest.raises(RuntimeError, match=words):
+            i8.int8_matmul(*args, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_matmul_witness_is_the_field_product(i8, layout):
+    from verinf_b200 import cuda_primitives as cp
+    g = torch.Generator().manual_seed(8)
+    A, B = _rand8(g, 200, 700).cuda(), _weight(g, 700, 333, layout, 0)
+    lift = lambda t: torch.where(t < 0, t.long() + (P - (1 << 64)), t.long()).contiguous().view(torch.uint64)
+    want = cp.gl_matmul(lift(A), lift(B))
+    assert torch.equal(i8.int8_matmul(A, B, dtype=torch.uint64).view(torch.int64), want.view(torch.int64))
+
+
+# ---- log probabilities ------------------------------------------------------------------------------------------------
+def _logprobs_64(x, tokens, top, temperature):
+    x = x.cpu().double()
+    rows, vocab = x.shape
+    tokens = tokens.cpu()
+    lp, ent = torch.zeros(rows, dtype=torch.float64), torch.zeros(rows, dtype=torch.float64)
+    tl, tt = torch.full((rows, top), -math.inf, dtype=torch.float64), torch.full((rows, top), -1, dtype=torch.int64)
+    log_z, width = torch.zeros(rows, dtype=torch.float64), torch.zeros(rows, dtype=torch.float64)
+    for r in range(rows):
+        v, t = x[r], int(tokens[r])
+        if torch.isnan(v).any() or (v == math.inf).any():
+            lp[r] = ent[r] = math.nan
+            tl[r] = math.nan
+        elif (v == -math.inf).all():
+            lp[r] = -math.inf
+        else:
+            z = (v - v.max()) / temperature
+            e = z.exp()
+            s = e.sum()
+            log_z[r] = s.log()
+            w = (e * torch.where(e > 0, z, 0.0)).sum() / s
+            width[r] = -w
+            ent[r] = s.log() - w
+            lp[r] = z[max(0, min(t, vocab - 1))] - s.log()
+            order = torch.sort(v, descending=True, stable=True)[1][:top]
+            order = order[v[order] > -math.inf]
+            tt[r, :len(order)] = order
+            tl[r, :len(order)] = z[order] - s.log()
+        if t < 0:
+            lp[r] = 0
+        elif t >= vocab:
+            lp[r] = math.nan
+    return lp, ent, tl, tt, log_z, width
+
+
+def _near(got, want, tol):
+    # the value is an fp32 number: one of more than 2^128 (1 - 2^-25) in size is infinite there, as -2 * 3.4e38 is
+    got, want = got.cpu().double(), want.float().double()
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    return bool((same | ((got - want).abs() <= tol)).all())
+
+
+def _check_logprobs(lp_mod, x, tokens, top=0, temperature=1.0):
+    out = lp_mod.token_logprobs(x, tokens, top=top, temperature=temperature)
+    lp, ent, tl, tt, log_z, width = _logprobs_64(x, tokens, top, temperature)
+    assert torch.equal(out.top_token.cpu(), tt)
+    # Half steps of fp32.  An exponential: its argument is a difference, a product and a rounded constant (3 half steps of
+    # |z|, and only |z| < 24 counts: the rest is below half a step of the sum) and the function itself (4).  The sum: one
+    # rounding a term of a thread's chain (vocab / 256 terms) and of the tree, rescaling included (64).  The logarithm and
+    # the difference: 4 each of their values; z of the token itself: 3.
+    u = HALF[torch.float32]
+    rel = (3 * 24 + 4 + x.size(1) / 256 + 64) * u
+    assert _near(out.logprob, lp, rel + u * (8 * log_z + 4 * torch.nan_to_num(lp, 0, 0, 0).abs()))
+    assert _near(out.entropy, ent, rel * (1 + 2 * width) + 8 * u * (log_z + width))
+    assert _near(out.top_logprob, tl, rel + u * (8 * log_z[:, None] + 4 * torch.nan_to_num(tl, 0, 0, 0).abs()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 2, 5), (2, 7, 32), (4, 8, 3), (2, 31, 8), (5, 255, 20), (9, 1000, 32), (3, 4099, 20),
+                                            (2, 32000, 20), (1, 70001, 32), (300, 513, 4), (2, 202045, 20), (2, 2048, 0)])
+def test_logprobs_sizes(lp, dtype, rows, vocab, top):
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, generator=g) * 3).to(dtype).cuda()
+    tokens = torch.randint(0, vocab, (rows,), generator=g).cuda()
+    _check_logprobs(lp, x, tokens, top)
+    _check_logprobs(lp, x, tokens, top, temperature=0.6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("low", ["inf", "lowest"])
+def test_logprobs_masks_and_special_rows(lp, dtype, low):
+    vocab, top = 3001, 20
+    g = torch.Generator().manual_seed(11)
+    low = -math.inf if low == "inf" else torch.finfo(dtype).min
+    x = (torch.randn(14, vocab, generator=g) * 4).to(dtype)
+    tokens = torch.randint(0, vocab, (14,), generator=g)
+    x[0, torch.rand(vocab, generator=g) < 0.9] = low
+    x[1] = low                                        # nothing left
+    x[2] = low; x[2, 1234] = 3.5                      # one token left, the one asked for or another
+    tokens[2] = 1234
+    x[3] = low; x[3, 77] = -20
+    x[4, 2000] = math.nan
+    x[5, 3000] = math.inf
+    x[6] = 1.25                                       # all alike
+    tokens[7] = -1
+    tokens[8] = vocab
+    tokens[9] = -100
+    x[10] = low; x[10, 5:12] = 0.5; x[10, 3000] = 0.5  # fewer than the list holds
+    x[11] = 0; x[11, ::3] = -0.0                      # equal zeros of either sign
+    x[12] = torch.finfo(dtype).max * torch.tensor([1, 0.5, -1]).repeat(vocab)[:vocab]
+    x[13] = torch.linspace(-9, 9, vocab)
+    _check_logprobs(lp, x.to(dtype).cuda(), tokens.cuda(), top)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_logprobs_orders_and_crowded_lists(lp, dtype):
+    """Rising and falling rows, runs of equal values, and rows whose allowed entries crowd in a few threads' shares."""
+    vocab = 70000
+    x = torch.full((7, vocab), -math.inf)
+    x[0] = torch.linspace(-5, 5, vocab)
+    x[1] = torch.linspace(5, -5, vocab)
+    x[2] = (torch.arange(vocab) // 100 % 7).float()
+    i = torch.arange(vocab)
+    for r, step in ((3, 512), (4, 1024), (5, 2048)):
+        at = i % step < 16
+        x[r, at] = torch.arange(int(at.sum())).float() / 512
+    x[6] = 2.0
+    tokens = torch.tensor([69999, 0, 5, 512, 1024, 2048, 33])
+    _check_logprobs(lp, x.to(dtype).cuda(), tokens.cuda(), 32)
+    _check_logprobs(lp, x.to(dtype).cuda(), tokens.cuda(), 1, temperature=2.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("offset,pitch", [(0, 4016), (0, 4003), (1, 4016), (8, 4016), (3, 4005)])
+def test_logprobs_strides(lp, dtype, offset, pitch):
+    g = torch.Generator().manual_seed(offset + pitch)
+    x = (torch.randn(6, pitch + 16, generator=g) * 3).to(dtype).cuda()
+    x[:, offset + 3999:] = 100.0                       # behind the vocabulary: must not be read as part of it
+    x[:, :offset] = 100.0
+    tokens = torch.randint(0, 3999, (6,), generator=g).cuda()
+    _check_logprobs(lp, x[:, offset:offset + 3999], tokens, 8)
+    _check_logprobs(lp, x[2:3, offset:offset + 3999].expand(5, 3999), tokens[:5].contiguous(), 3)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1e-6, 0.05, 30.0, 1e6])
+def test_logprobs_temperatures(lp, temperature):
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(4, 1500, generator=g) * 5
+    x[1] *= 1000
+    x[2] = (x[2] * 8).round() / 8
+    tokens = x.argmax(1)
+    tokens[3] = 7
+    out = lp.token_logprobs(x.cuda(), tokens.cuda(), top=5, temperature=temperature)
+    # c = 1 / T is rounded: a difference of |z| costs two more half steps, beside those counted for T = 1
+    w = _logprobs_64(x, tokens, 5, temperature)
+    u = HALF[torch.float32]
+    rel = (5 * 24 + 4 + 1500 / 256 + 64) * u
+    assert torch.equal(out.top_token.cpu(), w[3])
+    assert _near(out.logprob, w[0], rel + u * (8 * w[4] + 6 * w[0].abs()))
+    assert _near(out.entropy, w[1], rel * (1 + 2 * w[5]) + 8 * u * (w[4] + w[5]))
+    assert _near(out.top_logprob, w[2], rel + u * (8 * w[4][:, None] + 6 * w[2].abs()))
+
+
+@gpu
+def test_logprobs_refusals(lp):
+    x, t = torch.zeros(3, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    assert lp.token_logprobs(x[:0], t[:0], top=4).top_token.shape == (0, 4)
+    for args, kw, words in [((x.double(), t), {}, "dtype"), ((x[0], t), {}, "2-D"), ((x, t[:2]), {}, "tokens"), ((x, t.int()), {}, "tokens"),
+                            ((x, t.cpu()), {}, "tokens"), ((x, t), dict(top=33), "top"), ((x, t), dict(top=-1), "top"),
+                            ((x, t), dict(top=2.0), "top"), ((x, t), dict(temperature=0.0), "temperature"),
+                            ((x, t), dict(temperature=math.nan), "temperature"), ((torch.zeros(8, 3, device="cuda").t(), t), {}, "lie together"),
+                            ((x[:, :0], t), {}, "vocab")]:
+        with pytest.raises(RuntimeError, match=words):
+            lp.token_logprobs(*args, **kw)
+
+
+# ---- together, as they are used ------------------------------------------------------------------------------------------
+def _answer(i8, lp, hidden, weight, sw, tokens, out=None):
+    q, s = i8.int8_quantize_rows(hidden, out=out)
+    logits = i8.int8_matmul(q, weight.t(), s, sw, dtype=torch.float32)
+    witness = i8.int8_matmul(q, weight.t(), dtype=torch.uint64)
+    return (q, s, logits, witness) + tuple(lp.token_logprobs(logits, tokens, top=5))
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 9, 150])
+def test_answers_of_a_quantised_head(i8, lp, m):
+    """Hidden states to int8, the head product as logits and as witness, log probabilities of the answers: each against 64
+    bits from its own inputs, a second run on another stream and a captured and replayed one the same bit for bit."""
+    g = torch.Generator().manual_seed(m)
+    d, vocab = 1024, 5003
+    hidden = torch.randn(m, d, generator=g).bfloat16().cuda()
+    weight, sw = i8.int8_quantize_rows((torch.randn(vocab, d, generator=g) * 0.1).cuda())
+    tokens = torch.randint(0, vocab, (m,), generator=g).cuda()
+    first = _answer(i8, lp, hidden, weight, sw, tokens)
+    q, s, logits, witness = first[:4]
+    wq, ws = _quantize_64(hidden)
+    assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)
+    S = _sums_64(q, weight.t())
+    assert np.array_equal(witness.view(torch.int64).cpu().numpy(), _field(S))
+    want = S.double() * ws.double()[:, None] * sw.cpu().double()
+    assert ((logits.cpu().double() - want).abs() <= 3.01 * HALF[torch.float32] * want.abs()).all()
+    _check_logprobs(lp, logits, tokens, 5)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = _answer(i8, lp, hidden, weight, sw, tokens)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    inputs = torch.zeros_like(hidden)
+    with torch.cuda.graph(graph):
+        captured = _answer(i8, lp, inputs, weight, sw, tokens)
+    inputs.copy_(hidden)
+    graph.replay()
+    torch.cuda.synchronize()
+    as_bits = lambda t: t.view(torch.int64) if t.dtype == torch.uint64 else t
+    for a, b, c in zip(first, again, captured):
+        assert torch.equal(as_bits(a), as_bits(b)) and torch.equal(as_bits(a), as_bits(c))

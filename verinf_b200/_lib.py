@@ -3,6 +3,7 @@
 The library is the only compute path: if it is missing or fails to load, importing
 this module raises — there is no CPU or PyTorch fallback.
 """
+import contextlib
 import ctypes as C
 import os
 from pathlib import Path
@@ -74,6 +75,9 @@ SIGNATURES = {
     "vi_lookup_multiplicities": (_int, [_p, _i64, _p, _i64, _p, _p]),
     "vi_interp_band": (_int, [_int, _p, _i64, _i64, _i64, _u64, _u64, _u64, _u64,
                               _p, _p, _p, _p, _i64, _p, _p, _int, _p]),
+    "vi_int8_quantize_rows": (_int, [_p, _int, _i64, _i64, _i64, _p, _i64, _p, _p]),
+    "vi_int8_matmul": (_int, [_p, _i64, _p, _i64, _int, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p]),
+    "vi_token_logprobs": (_int, [_p, _int, _i64, _i64, _i64, _p, _int, C.c_float, _p, _p, _p, _p, _p]),
     "vi_profile_enable": (None, [_int]),
     "vi_profile_num_tags": (_int, []),
     "vi_profile_tag_name": (C.c_char_p, [_int]),
@@ -104,6 +108,19 @@ def check(rc: int) -> None:
 
 def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+_NOTHING = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which `device` is current: torch.cuda.device, skipped where it is current already."""
+    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def raw_stream(device) -> int:
+    """torch's current stream of `device`."""
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def ptr(t) -> int:

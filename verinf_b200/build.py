@@ -7,7 +7,8 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 SO = HERE / "libverinf_b200.so"
-SOURCES = ["common.cu", "ntt.cu", "hash.cu", "field_ops.cu", "kquant.cu", "sumcheck.cu", "sumcheck_prove.cu", "open.cu", "matmul_tc.cu", "matmul_umma.cu"]
+SOURCES = ["common.cu", "ntt.cu", "hash.cu", "field_ops.cu", "kquant.cu", "sumcheck.cu", "sumcheck_prove.cu", "open.cu", "matmul_tc.cu", "matmul_umma.cu",
+           "int8_quant.cu", "int8_matmul.cu", "logprobs.cu"]
 # One compilation per source: with --split-compile two builds of ntt.cu differed in the registers or spills of half their
 # kernels, and its short tiles by 8 % in time.
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
