@@ -336,10 +336,17 @@ int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_
  * apart, or, with b_by_channel, stored (n, k) with the k values of a channel together and channels ldb bytes apart.
  * out_type VI_F32 / VI_F16 / VI_BF16: C_ij = (S_ij * sa_i) * sb_j in fp32, rounded once to the type (sa (m), sb (n); NULL =
  * ones); VI_I32: S; VI_FIELD: S mod p as uint64_t, negative sums as p - |S| (the same value vi_gl_matmul gives for the
- * lifted operands); these two take no scales.  C rows ldc elements apart. */
+ * lifted operands); these two take no scales.  C rows ldc elements apart; C must not overlap an operand.
+ * An operand whose rows (channels) all start on 16-byte boundaries is read in place, another one is first copied to the
+ * scratch: vi_int8_matmul_scratch_bytes (0 when both are read in place), 16-byte aligned.
+ * vi_int8_matmul_status: *code = non-zero if a product on the current device gave up on one of its bounded waits since the
+ * last call (its output is then incomplete); waits for the device. */
+int64_t vi_int8_matmul_scratch_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel,
+                                     int64_t m, int64_t k, int64_t n);
 int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel,
                    const float* sa, const float* sb, void* C, int out_type, int64_t ldc,
-                   int64_t m, int64_t k, int64_t n, void* stream);
+                   int64_t m, int64_t k, int64_t n, void* scratch, int64_t scratch_bytes, void* stream);
+int vi_int8_matmul_status(int* code);
 
 /* What each row of logits (rows x vocab, `stride` elements apart, VI_F32 / VI_F16 / VI_BF16) says about its token, with
  * p = softmax(x / temperature): logprob[r] = log p[tokens[r]] (0 where the token is negative: no token at this position;

@@ -62,7 +62,7 @@ def test_matmul_refusals_without_gpu(lib):
     keep, p = _buf()
 
     def call(A=p, lda=4, B=p, ldb=4, nk=0, sa=None, sb=None, Cp=p, out=3, ldc=4, m=2, k=4, n=4):
-        return L.vi_int8_matmul(A, lda, B, ldb, nk, sa, sb, Cp, out, ldc, m, k, n, None)
+        return L.vi_int8_matmul(A, lda, B, ldb, nk, sa, sb, Cp, out, ldc, m, k, n, None, 0, None)
     assert call(m=-1) != 0 and "negative" in _err(lib)
     assert call(out=5) != 0 and "output type" in _err(lib)
     assert call(out=-1) != 0 and "output type" in _err(lib)
@@ -74,6 +74,12 @@ def test_matmul_refusals_without_gpu(lib):
     assert call(ldc=3) != 0 and "overlap" in _err(lib)
     assert call(A=None) != 0 and "null input" in _err(lib)
     assert call(out=0, sa=p + 1) != 0 and "scales" in _err(lib)
+    assert call(lda=3) != 0 and "operand rows overlap" in _err(lib)
+    assert call(nk=1, k=5, lda=5) != 0 and "operand rows overlap" in _err(lib)
+    assert call(A=p + 1) != 0 and "scratch" in _err(lib)
+    assert L.vi_int8_matmul_scratch_bytes(16, 16, 32, 16, 0, 2, 4, 4) == 0
+    assert L.vi_int8_matmul_scratch_bytes(16, 17, 33, 16, 1, 2, 17, 5) == 2 * 32 + 5 * 32
+    assert L.vi_int8_matmul_status(None) != 0 and "null" in _err(lib)
     assert call(m=0, A=None, Cp=None) == 0
     assert call(n=0, A=None, Cp=None) == 0
 

@@ -8,70 +8,265 @@
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
 #include "gl.cuh"
+#include "umma.cuh"
 
 namespace {
+
+using namespace vumma;
 
 constexpr int64_t I8_MAX_K = 131071;
 
 template <typename T> struct Out;
-template <> struct Out<float> { static __device__ __forceinline__ float make(int s, float sc) { return (float)s * sc; } };
-template <> struct Out<__half> { static __device__ __forceinline__ __half make(int s, float sc) { return __float2half_rn((float)s * sc); } };
-template <> struct Out<__nv_bfloat16> { static __device__ __forceinline__ __nv_bfloat16 make(int s, float sc) { return __float2bfloat16_rn((float)s * sc); } };
-template <> struct Out<int32_t> { static __device__ __forceinline__ int32_t make(int s, float) { return s; } };
+template <> struct Out<float> { static __device__ __forceinline__ float make(int s, float a, float b) { return (float)s * a * b; } };
+template <> struct Out<__half> { static __device__ __forceinline__ __half make(int s, float a, float b) { return __float2half_rn((float)s * a * b); } };
+template <> struct Out<__nv_bfloat16> { static __device__ __forceinline__ __nv_bfloat16 make(int s, float a, float b) { return __float2bfloat16_rn((float)s * a * b); } };
+template <> struct Out<int32_t> { static __device__ __forceinline__ int32_t make(int s, float, float) { return s; } };
 // p - |s| = s - (2^32 - 1) in 64-bit words
-template <> struct Out<uint64_t> { static __device__ __forceinline__ uint64_t make(int s, float) { return (uint64_t)(int64_t)s - (s < 0 ? vgl::EPS : 0ull); } };
+template <> struct Out<uint64_t> { static __device__ __forceinline__ uint64_t make(int s, float, float) { return (uint64_t)(int64_t)s - (s < 0 ? vgl::EPS : 0ull); } };
 
-// 64 x 64 outputs a block, 4 x 4 a thread, slices of 32 terms in shared memory, four products an instruction.
-template <typename T>
-__global__ void __launch_bounds__(256) k_int8_tile(const int8_t* __restrict__ A, int64_t lda, const int8_t* __restrict__ B, int64_t bk, int64_t bn,
-                                                   const float* __restrict__ sa, const float* __restrict__ sb, T* __restrict__ C, int64_t ldc,
-                                                   int64_t m, int64_t k, int64_t n) {
-    __shared__ int As[64][9], Bs[64][9];
-    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    int acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < k; k0 += 32) {
-        for (int i = tid; i < 64 * 32; i += 256) {
-            const int64_t r = r0 + (i >> 5), kk = k0 + (i & 31);
-            reinterpret_cast<int8_t*>(&As[i >> 5][0])[i & 31] = r < m && kk < k ? A[r * lda + kk] : (int8_t)0;
-            const int cl = bn == 1 ? (i & 63) : (i >> 5), kl = bn == 1 ? (i >> 6) : (i & 31);      // neighbours read neighbours
-            const int64_t c = c0 + cl, kb = k0 + kl;
-            reinterpret_cast<int8_t*>(&Bs[cl][0])[kl] = c < n && kb < k ? B[kb * bk + c * bn] : (int8_t)0;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            int a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { a[i] = As[ty + 16 * i][w]; b[i] = Bs[tx + 16 * i][w]; }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[i], b[j], acc[i][j]);
-        }
-        __syncthreads();
+// ---- tcgen05 ---------------------------------------------------------------------------------------------------
+// A tile is 128 channels by `nt` tokens: the weight is the operand with 128 rows, so a lane of tensor memory is a channel, a
+// column a token, and a warp writes 32 neighbouring channels of one token.
+constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 12;
+constexpr int I8_W_BYTES = I8_TN * I8_KS;
+constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, tensor-memory slot, scales of the tokens
+
+__device__ int g_i8_status;                                          // first wait that expired, 0 = none
+
+struct Plan { int nt, split, stages; };
+__host__ __device__ inline int i8_stage_bytes(int nt) { return I8_W_BYTES + nt * I8_KS; }
+
+// 128-byte rows, 128-byte swizzle, groups of 8 rows 1024 bytes apart: K-major tiles (rows = channels or tokens), and tiles
+// of a row-major weight (rows = terms; one atom is 128 channels wide, so the leading offset is never used).
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// s8 x s8 -> s32; bit 15: the first operand is MN-major
+__device__ __forceinline__ uint32_t idesc_s8(int nt, bool kn) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (kn ? 1u << 15 : 0u) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(I8_TN >> 4) << 24);
+}
+
+enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
+
+// One tile a block, or, with split > 1, one tile a cluster whose blocks each take a share of the terms; the sums meet through
+// distributed shared memory (whole numbers: the order does not matter).
+template <typename T, bool KN>
+__global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                          const float* __restrict__ sa, const float* __restrict__ sb, T* __restrict__ C, int64_t ldc,
+                                                          int64_t m, int64_t n, int t_tiles, int slices, int nt, int split, int stages) {
+    extern __shared__ uint8_t i8_raw[];
+    uint8_t* base = (uint8_t*)(((uintptr_t)i8_raw + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = i8_stage_bytes(nt);
+    uint64_t* bars = (uint64_t*)(base + stages * stage_bytes);
+    float* sa_s = (float*)(bars + 2 * I8_MAX_STAGES + 8);
+    volatile uint32_t* tmem_slot = (volatile uint32_t*)(bars + 2 * I8_MAX_STAGES + 1);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    const uint32_t ring = smem_u32(base), full0 = smem_u32(bars), empty0 = smem_u32(bars + I8_MAX_STAGES), accb = smem_u32(bars + 2 * I8_MAX_STAGES);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)blockIdx.x % split, tile = (int)blockIdx.x / split;
+    const int64_t n0 = (int64_t)(tile / t_tiles) * I8_TN, m0 = (int64_t)(tile % t_tiles) * nt;
+    const int s0 = (int)((int64_t)slices * rank / split), s1 = (int)((int64_t)slices * (rank + 1) / split);
+    uint32_t cols = 32;
+    while ((int)cols < nt) cols <<= 1;
+
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        mbar_init(accb, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = r0 + ty + 16 * i, c = c0 + tx + 16 * j;
-            if (r < m && c < n) C[r * ldc + c] = Out<T>::make(acc[i][j], (sa ? sa[r] : 1.0f) * (sb ? sb[c] : 1.0f));
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    for (int j = tid; j < nt; j += I8_THREADS) sa_s[j] = sa && m0 + j < m ? sa[m0 + j] : 1.0f;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int st = 0;
+        uint32_t par = 0;
+        for (int s = s0; s < s1; ++s) {
+            if (s - s0 >= stages && !mbar_wait_soon(empty0 + 8 * st, par ^ 1)) { *abort_flag = I8_ERR_EMPTY; break; }
+            const uint32_t fb = full0 + 8 * st, dst = ring + st * stage_bytes;
+            mbar_expect_tx(fb, stage_bytes);
+            if (KN) tma_load_2d(dst, &map_w, (int32_t)n0, s * I8_KS, fb);
+            else tma_load_2d(dst, &map_w, s * I8_KS, (int32_t)n0, fb);
+            tma_load_2d(dst + I8_W_BYTES, &map_x, s * I8_KS, (int32_t)m0, fb);
+            if (++st == stages) { st = 0; par ^= 1; }
         }
+    } else if (warp == 1 && lane == 0) {
+        int st = 0;
+        uint32_t par = 0;
+        const uint32_t idesc = idesc_s8(nt, KN);
+        for (int s = s0; s < s1 && !*abort_flag; ++s) {
+            if (!mbar_wait_soon(full0 + 8 * st, par)) { *abort_flag = I8_ERR_FULL; break; }
+            tc_fence_after();
+            const uint32_t w = ring + st * stage_bytes, x = w + I8_W_BYTES;
+#pragma unroll
+            for (int kk = 0; kk < I8_KS / 32; ++kk)
+                umma_i8(tmem, desc_sw128(w + kk * (KN ? 32 * 128 : 32)), desc_sw128(x + kk * 32), idesc, s > s0 || kk > 0);
+            umma_commit(empty0 + 8 * st);
+            if (s + 1 == s1) umma_commit(accb);
+            if (++st == stages) { st = 0; par ^= 1; }
+        }
+    }
+    __syncwarp();
+    bool ok = mbar_wait_soon(accb, 0);
+    if (!ok && *abort_flag == 0) *abort_flag = I8_ERR_ACC;
+    tc_fence_after();
+    ok = ok && *abort_flag == 0;
+    const int quad = warp & 3, half = warp >> 2;
+    const int64_t ch = n0 + 32 * quad + lane;
+    const float sbv = sb && ch < n ? sb[ch] : 1.0f;
+    auto put = [&](int j, uint32_t v) {
+        if (ch < n && m0 + j < m) C[(m0 + j) * ldc + ch] = Out<T>::make((int)v, sa_s[j], sbv);
+    };
+    if (ok) {
+        for (int q = half; q < nt / 16; q += 2) {
+            uint32_t r[16];
+            tmem_ld16(tmem + ((uint32_t)(32 * quad) << 16) + 16 * q, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (split == 1) put(16 * q + j, r[j]);
+                else ((uint32_t*)base)[(16 * q + j) * I8_TN + 32 * quad + lane] = r[j];
+            }
+        }
+    }
+    if (split > 1) {
+        __syncwarp();
+        cluster_sync();
+        const int per = nt / split;
+        if (ok) {
+            for (int j = rank * per + half; j < (rank + 1) * per; j += 2) {
+                uint32_t v = 0;
+                for (int p = 0; p < split; ++p) v += cluster_ld(ring + (j * I8_TN + 32 * quad + lane) * 4, p);
+                put(j, v);
+            }
+        }
+        __syncwarp();
+        cluster_sync();            // no block leaves while another reads its sums
+    }
+    if (*abort_flag) {
+        if (tid == 0) atomicCAS(&g_i8_status, 0, (int)*abort_flag);
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);        // copies in flight land in this block's shared memory
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
+// rows x len bytes, rows `pitch` bytes apart; box: 128 bytes x box_rows
+int make_map(CUtensorMap* map, const int8_t* ptr, int64_t rows, int64_t len, int64_t pitch, int box_rows) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return vi::fail(VI_ERR_CUDA, "int8_matmul: cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)len, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)I8_KS, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return vi::fail(VI_ERR_CUDA, "int8_matmul: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return VI_OK;
+}
+
+struct Product {
+    const int8_t *A, *B;
+    int64_t lda, ldb;
+    bool by_channel;
+    const float *sa, *sb;
+    void* C;
+    int64_t ldc, m, k, n;
+};
+
+template <typename T, bool KN>
+int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
+    CUtensorMap map_w, map_x;
+    int rc = KN ? make_map(&map_w, p.B, p.k, p.n, p.ldb, I8_KS) : make_map(&map_w, p.B, p.n, p.k, p.ldb, I8_TN);
+    if (rc) return rc;
+    rc = make_map(&map_x, p.A, p.m, p.k, p.lda, plan.nt);
+    if (rc) return rc;
+    const int smem = plan.stages * i8_stage_bytes(plan.nt) + 1024 + I8_TAIL;
+    VI_CUDA(cudaFuncSetAttribute(k_int8_umma<T, KN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, n_tiles = (p.n + I8_TN - 1) / I8_TN;
+    VI_REQUIRE(t_tiles * n_tiles * plan.split <= 0x7FFFFFFF, "int8_matmul: matrix too large for one launch");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(t_tiles * n_tiles * plan.split));
+    cfg.blockDim = dim3(I8_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)plan.split, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = plan.split > 1 ? 1 : 0;
+    VI_CUDA(cudaLaunchKernelEx(&cfg, k_int8_umma<T, KN>, map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles,
+                               (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.split, plan.stages));
+    return VI_OK;
 }
 
 template <typename T>
-int launch_tile(const int8_t* A, int64_t lda, const int8_t* B, int64_t bk, int64_t bn, const float* sa, const float* sb, void* C, int64_t ldc,
-                int64_t m, int64_t k, int64_t n, cudaStream_t st) {
-    dim3 grid((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64));
-    k_int8_tile<T><<<grid, 256, 0, st>>>(A, lda, B, bk, bn, sa, sb, (T*)C, ldc, m, k, n);
-    return vi::check_launch("k_int8_tile");
+int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
+    return p.by_channel ? launch_umma<T, false>(p, plan, st) : launch_umma<T, true>(p, plan, st);
+}
+
+Plan make_plan(int64_t m, int64_t k, int64_t n) {
+    Plan p;
+    p.nt = m >= 256 ? 256 : (int)((m + 15) / 16 * 16);
+    const int64_t slices = (k + I8_KS - 1) / I8_KS, tiles = ((m + p.nt - 1) / p.nt) * ((n + I8_TN - 1) / I8_TN);
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split < 148 && slices >= 8 * p.split) p.split *= 2;
+    p.stages = (p.nt <= 32 ? 110 : 200) * 1024 / i8_stage_bytes(p.nt);
+    if (p.stages > I8_MAX_STAGES) p.stages = I8_MAX_STAGES;
+    return p;
+}
+
+// ---- operands that TMA cannot read in place -----------------------------------------------------------------------
+// Rows that start off the 16-byte grid are copied to rows that start on it (a pass over those bytes; the caller's rows are
+// copied anew on every call).
+__global__ void __launch_bounds__(256) k_int8_align(const int8_t* __restrict__ src, int64_t pitch, int64_t rows, int64_t len, int8_t* __restrict__ dst, int64_t dst_pitch) {
+    const int64_t per = dst_pitch / 4, total = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per, c = (i % per) * 4;
+        uint32_t v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < len) v |= (uint32_t)(uint8_t)src[r * pitch + c + e] << (8 * e);
+        *(uint32_t*)(dst + r * dst_pitch + c) = v;
+    }
+}
+
+inline int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
+inline bool in_place(const void* p, int64_t pitch) { return ((uintptr_t)p) % 16 == 0 && pitch % 16 == 0; }
+inline int64_t b_rows(int64_t k, int64_t n, bool by_channel) { return by_channel ? n : k; }
+inline int64_t b_len(int64_t k, int64_t n, bool by_channel) { return by_channel ? k : n; }
+
+int align_rows(const int8_t*& ptr, int64_t& pitch, int64_t rows, int64_t len, int8_t*& room, cudaStream_t st) {
+    if (in_place(ptr, pitch)) return VI_OK;
+    const int64_t to = up16(len), words = rows * (to / 4), want = (words + 255) / 256;
+    k_int8_align<<<(unsigned)(want < 148 * 16 ? want : 148 * 16), 256, 0, st>>>(ptr, pitch, rows, len, room, to);
+    ptr = room;
+    pitch = to;
+    room += rows * to;
+    return vi::check_launch("k_int8_align");
 }
 
 }  // namespace
 
+extern "C" int64_t vi_int8_matmul_scratch_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel, int64_t m, int64_t k, int64_t n) {
+    if (m <= 0 || k <= 0 || n <= 0) return 0;
+    if (m == 1) lda = 16;                                            // a single row has no next one
+    if (b_rows(k, n, b_by_channel != 0) == 1) ldb = 16;
+    return (in_place(A, lda) ? 0 : m * up16(k)) +
+           (in_place(B, ldb) ? 0 : b_rows(k, n, b_by_channel != 0) * up16(b_len(k, n, b_by_channel != 0)));
+}
+
 extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel, const float* sa, const float* sb,
-                              void* C, int out_type, int64_t ldc, int64_t m, int64_t k, int64_t n, void* stream) {
+                              void* C, int out_type, int64_t ldc, int64_t m, int64_t k, int64_t n, void* scratch, int64_t scratch_bytes,
+                              void* stream) {
     VI_REQUIRE(m >= 0 && k >= 0 && n >= 0, "int8_matmul: negative size");
     VI_REQUIRE(out_type >= VI_F32 && out_type <= VI_FIELD, "int8_matmul: unknown output type");
     VI_REQUIRE(k <= I8_MAX_K, "int8_matmul: k = %lld, but 32-bit sums hold at most 131071 products", (long long)k);
@@ -82,14 +277,41 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     VI_REQUIRE(m == 1 || ldc >= n, "int8_matmul: output rows overlap (stride below n)");
     VI_REQUIRE(k == 0 || (A && B), "int8_matmul: null input");
     VI_REQUIRE(((uintptr_t)sa) % 4 == 0 && ((uintptr_t)sb) % 4 == 0, "int8_matmul: misaligned scales");
-    VI_REQUIRE((m + 63) / 64 <= 65535 && (n + 63) / 64 <= 0x7FFFFFFF, "int8_matmul: matrix too large for one launch");
+    VI_REQUIRE(m < (int64_t(1) << 31) && n < (int64_t(1) << 31), "int8_matmul: m and n are limited to 2^31 - 1");
     cudaStream_t st = (cudaStream_t)stream;
-    const int64_t bk = b_by_channel ? 1 : ldb, bn = b_by_channel ? ldb : 1;
-    switch (out_type) {
-        case VI_F32: return launch_tile<float>(A, lda, B, bk, bn, sa, sb, C, ldc, m, k, n, st);
-        case VI_F16: return launch_tile<__half>(A, lda, B, bk, bn, sa, sb, C, ldc, m, k, n, st);
-        case VI_BF16: return launch_tile<__nv_bfloat16>(A, lda, B, bk, bn, sa, sb, C, ldc, m, k, n, st);
-        case VI_I32: return launch_tile<int32_t>(A, lda, B, bk, bn, sa, sb, C, ldc, m, k, n, st);
-        default: return launch_tile<uint64_t>(A, lda, B, bk, bn, sa, sb, C, ldc, m, k, n, st);
+    if (k == 0) {
+        VI_CUDA(cudaMemset2DAsync(C, (size_t)(ldc * out_bytes[out_type]), 0, (size_t)(n * out_bytes[out_type]), (size_t)m, st));
+        return VI_OK;
     }
+    const bool nk = b_by_channel != 0;
+    if (m == 1) lda = up16(k);
+    if (b_rows(k, n, nk) == 1) ldb = up16(b_len(k, n, nk));
+    VI_REQUIRE(lda >= k && ldb >= b_len(k, n, nk), "int8_matmul: operand rows overlap");
+    VI_REQUIRE(lda < (int64_t(1) << 40) && ldb < (int64_t(1) << 40), "int8_matmul: rows too far apart");
+    const int64_t need = vi_int8_matmul_scratch_bytes(A, lda, B, ldb, b_by_channel, m, k, n);
+    if (need && (scratch == nullptr || scratch_bytes < need))
+        return vi::fail(VI_ERR_SCRATCH, "int8_matmul: scratch of at least %lld bytes required (see vi_int8_matmul_scratch_bytes)", (long long)need);
+    VI_REQUIRE(!need || ((uintptr_t)scratch) % 16 == 0, "int8_matmul: scratch must be 16-byte aligned");
+    int8_t* room = (int8_t*)scratch;
+    int rc = align_rows(A, lda, m, k, room, st);
+    if (rc) return rc;
+    rc = align_rows(B, ldb, b_rows(k, n, nk), b_len(k, n, nk), room, st);
+    if (rc) return rc;
+    const Product p = {A, B, lda, ldb, nk, sa, sb, C, ldc, m, k, n};
+    const Plan plan = make_plan(m, k, n);
+    switch (out_type) {
+        case VI_F32: return launch_umma<float>(p, plan, st);
+        case VI_F16: return launch_umma<__half>(p, plan, st);
+        case VI_BF16: return launch_umma<__nv_bfloat16>(p, plan, st);
+        case VI_I32: return launch_umma<int32_t>(p, plan, st);
+        default: return launch_umma<uint64_t>(p, plan, st);
+    }
+}
+
+extern "C" int vi_int8_matmul_status(int* code) {
+    VI_REQUIRE(code, "int8_matmul_status: null pointer");
+    const int none = 0;
+    VI_CUDA(cudaMemcpyFromSymbol(code, g_i8_status, sizeof(int)));
+    if (*code) VI_CUDA(cudaMemcpyToSymbol(g_i8_status, &none, sizeof(int)));
+    return VI_OK;
 }

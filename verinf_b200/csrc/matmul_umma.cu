@@ -20,14 +20,15 @@
 //    accumulators; 8 warps read them back with tcgen05.ld and fold the 15 sums.
 //  * Every wait is bounded: on expiry the kernel records a code in `status`, lets copies in flight
 //    land, frees its tensor memory and returns.
-#include <cuda.h>
-
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
 #include "gl.cuh"
 #include "plane_fold.cuh"
+#include "umma.cuh"
 
 namespace {
+
+using namespace vumma;
 
 constexpr int UM_TM = 128, UM_TN = 32, UM_KS = 64;        // CTA tile, k bytes per stage
 constexpr int UM_STAGES = 2;
@@ -39,7 +40,6 @@ constexpr int UM_SMEM = UM_STAGES * UM_STAGE_BYTES + 1024 /* alignment slack */ 
 constexpr int64_t UM_KCHUNK = 4096;                        // 8 * 4096 * 255^2 < 2^31
 constexpr int UM_THREADS = 256;
 constexpr uint32_t UM_TMEM_COLS = 512;
-constexpr unsigned long long UM_WAIT_NS = 2000000000ull;   // a wait gives up after two seconds
 
 __host__ __device__ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -77,55 +77,6 @@ __global__ void __launch_bounds__(256) k_um_split_cols(const uint64_t* __restric
     }
 }
 
-// ---- PTX wrappers -----------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ unsigned long long global_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// bounded wait for the phase with the given parity to complete (non-blocking test, short sleeps);
-// false = gave up after UM_WAIT_NS
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    const unsigned long long t0 = global_ns();
-    for (uint32_t it = 0;; ++it) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
-        if (it > 64) __nanosleep(64);
-        if ((it & 1023) == 1023 && global_ns() - t0 > UM_WAIT_NS) return false;
-    }
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t"
-                 "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
 // Shared-memory matrix descriptor of a K-major tile with 64-byte rows and the 64-byte swizzle: groups of
 // 8 rows are 512 bytes apart (stride offset), the leading offset is the canonical 1, version 1 (sm_100).
 __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr) {
@@ -136,7 +87,6 @@ __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr) {
 __host__ __device__ constexpr uint32_t idesc_u8(int n) {
     return (2u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(UM_TM >> 4) << 24);
 }
-
 
 enum { UM_ERR_FULL = 1, UM_ERR_EMPTY = 2, UM_ERR_ACC = 3 };
 
@@ -267,18 +217,6 @@ k_matmul_umma(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ 
     }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess) return (EncodeTiledFn) nullptr;
-        return q == cudaDriverEntryPointSuccess ? (EncodeTiledFn)p : (EncodeTiledFn) nullptr;
-    }();
-    return fn;
-}
 // 2-D byte tensor (rows x k_pad, row pitch k_pad), box of box_rows x 64 bytes, 64-byte swizzle
 int make_plane_map(CUtensorMap* map, uint8_t* ptr, int64_t rows, int64_t k_pad, uint32_t box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();

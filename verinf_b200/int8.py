@@ -8,6 +8,8 @@ one pass over one byte plane instead of 64 plane products.
 As elsewhere in the package: CUDA tensors, outputs allocated with torch (or given as `out`), kernels on torch's current stream
 of the tensors' device, RuntimeError for what is refused.
 """
+import ctypes as C
+
 import torch
 
 from ._lib import LIB, check, on_device, raw_stream
@@ -126,7 +128,22 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
         ldc = _rows_apart(out, what, "out")
         if ldc < n:
             raise RuntimeError(f"{what}: rows of out overlap")
+    a, b = A.data_ptr(), B.data_ptr()
+    room, nb = None, LIB.vi_int8_matmul_scratch_bytes(a, lda, b, ldb, by_channel, m, k, n)
+    if nb:
+        room = torch.empty((nb,), dtype=torch.int8, device=dev)      # of the current stream: calls on two streams share nothing
     with on_device(dev):
-        check(LIB.vi_int8_matmul(A.data_ptr(), lda, B.data_ptr(), ldb, by_channel, sa, sb, out.data_ptr(), DTYPE_CODES[dtype], ldc,
-                                 m, k, n, raw_stream(dev)))
+        check(LIB.vi_int8_matmul(a, lda, b, ldb, by_channel, sa, sb, out.data_ptr(), DTYPE_CODES[dtype], ldc, m, k, n,
+                                 room.data_ptr() if nb else None, nb, raw_stream(dev)))
     return out
+
+
+def check_async_errors(device=None):
+    """Raises if a product launched earlier on the device gave up on one of its bounded device-side waits (its output is then
+    incomplete).  Waits for the device."""
+    code = C.c_int(0)
+    with torch.cuda.device(device):
+        check(LIB.vi_int8_matmul_status(C.byref(code)))
+    if code.value:
+        raise RuntimeError(f"int8_matmul: a device-side wait expired (code {code.value}); the product written by that call is "
+                           "incomplete")
