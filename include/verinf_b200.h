@@ -325,7 +325,7 @@ int vi_interp_band(int kind, uint64_t* out, int64_t out_off, int64_t flat_lo, in
  * multiply them as field elements (gl_matmul).  Element types of inputs and outputs: */
 enum { VI_F32 = 0, VI_F16 = 1, VI_BF16 = 2, VI_I32 = 3, VI_FIELD = 4 };
 
-/* Rows to int8 with one scale a row: x (m, k) of VI_F32 / VI_F16 / VI_BF16, rows x_stride elements apart;
+/* Rows to int8 with one scale a row: x (m, k) of VI_F32 / VI_F16 / VI_BF16, rows x_stride elements apart (0: the same row);
  * scale[r] = max_j |x_rj| / 127, q_rj = the whole number nearest to 127 x_rj / max_j |x_rj| (of the exact quotient, ties
  * to even), in rows q_stride bytes apart.  A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN and
  * q = 0. */

@@ -49,7 +49,7 @@ def test_quantize_refusals_without_gpu(lib):
     assert L.vi_int8_quantize_rows(p, 3, 1, 4, 4, p, 4, p, None) != 0 and "dtype" in _err(lib)
     assert L.vi_int8_quantize_rows(p, 0, -1, 4, 4, p, 4, p, None) != 0 and "negative" in _err(lib)
     assert L.vi_int8_quantize_rows(p, 0, 1 << 31, 4, 4, p, 4, p, None) != 0 and "rows" in _err(lib)
-    assert L.vi_int8_quantize_rows(p, 0, 2, 4, 3, p, 4, p, None) != 0 and "overlap" in _err(lib)
+    assert L.vi_int8_quantize_rows(p, 0, 2, 4, -4, p, 4, p, None) != 0 and "negative" in _err(lib)
     assert L.vi_int8_quantize_rows(p, 0, 2, 4, 4, p, 3, p, None) != 0 and "overlap" in _err(lib)
     assert L.vi_int8_quantize_rows(p + 2, 0, 1, 4, 4, p, 4, p, None) != 0 and "aligned" in _err(lib)
     assert L.vi_int8_quantize_rows(p, 0, 1, 4, 4, p, 4, None, None) != 0 and "scale" in _err(lib)
@@ -213,7 +213,7 @@ def test_quantize_empty_and_refusals(i8):
     for bad, words in [((x.double(),), "dtype"), ((x[0],), "2-D"), ((x.t(),), "lie together")]:
         with pytest.raises(RuntimeError, match=words):
             i8.int8_quantize_rows(*bad)
-    for out, words in [((q[:3], s), "shape"), ((q.to(torch.int32), s), "dtype"), ((q[:1].expand(4, 6), s), "overlap"),
+    for out, words in [((q[:3], s), "must be 4 x 6"), ((q.to(torch.int32), s), "dtype"), ((q[:1].expand(4, 6), s), "overlap"),
                        ((q, s[:3]), "scales"), ((q, s.double()), "scales"), ((q, s.cpu()), "scales"), ((q.cpu(), s), "CUDA"),
                        ((torch.empty(6, 4, dtype=torch.int8, device="cuda").t(), s), "lie together")]:
         with pytest.raises(RuntimeError, match=words):

@@ -115,14 +115,14 @@ def stream_ptr() -> int:
 _NOTHING = contextlib.nullcontext()
 
 
-def on_device(device):
-    """Context in which `device` is current: torch.cuda.device, skipped where it is current already."""
-    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def on_device(index: int):
+    """Context in which the device of this index is current: torch.cuda.device, skipped where it is current already."""
+    return _NOTHING if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
-def raw_stream(device) -> int:
-    """torch's current stream of `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+# torch's current stream of a device index as a number, without the Stream object that torch.cuda.current_stream builds
+# (0.1 us instead of 2.2 us, of some 10 us that a small call takes)
+raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def ptr(t) -> int:

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
 #include "gl.cuh"
@@ -15,6 +17,7 @@ namespace {
 using namespace vumma;
 
 constexpr int64_t I8_MAX_K = 131071;
+constexpr int I8_MAX_SMEM = 227 * 1024;
 
 template <typename T> struct Out;
 template <> struct Out<float> { static __device__ __forceinline__ float make(int s, float a, float b) { return (float)s * a * b; } };
@@ -33,7 +36,7 @@ constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, 
 
 __device__ int g_i8_status;                                          // first wait that expired, 0 = none
 
-struct Plan { int nt, split, stages; };
+struct Plan { bool pair; int nt, split, stages; };
 __host__ __device__ inline int i8_stage_bytes(int nt) { return I8_W_BYTES + nt * I8_KS; }
 
 // 128-byte rows, 128-byte swizzle, groups of 8 rows 1024 bytes apart: K-major tiles (rows = channels or tokens), and tiles
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
 #pragma unroll
             for (int kk = 0; kk < I8_KS / 32; ++kk)
                 umma_i8(tmem, desc_sw128(w + kk * (KN ? 32 * 128 : 32)), desc_sw128(x + kk * 32), idesc, s > s0 || kk > 0);
-            umma_commit(empty0 + 8 * st);
+            if (s + stages < s1) umma_commit(empty0 + 8 * st);        // the last ones are not loaded again
             if (s + 1 == s1) umma_commit(accb);
             if (++st == stages) { st = 0; par ^= 1; }
         }
@@ -159,6 +162,135 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
+// ---- pairs of blocks, persistent --------------------------------------------------------------------------------
+// A tile is 256 channels by `nt` tokens, 128 channels a block; each block brings its channels and half of the tokens, so that
+// the tokens cross from L2 once a pair.  Two accumulators a block (2 x 256 columns of tensor memory): while eight warps write
+// one tile out, the products of the next one run.
+constexpr int I8_PAIR_THREADS = 320, I8_PAIR_STAGES = 8;
+constexpr int I8_PAIR_TAIL = (2 * I8_PAIR_STAGES + 4 + 1) * 8 + 24;
+__host__ __device__ inline int i8_pair_stage_bytes(int nt) { return I8_W_BYTES + nt / 2 * I8_KS; }
+
+template <typename T, bool KN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_PAIR_THREADS)
+k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ sa,
+            const float* __restrict__ sb, T* __restrict__ C, int64_t ldc, int64_t m, int64_t n, int t_tiles, int tiles, int slices, int nt, int stages) {
+    extern __shared__ uint8_t i8_raw[];
+    uint8_t* base = (uint8_t*)(((uintptr_t)i8_raw + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = i8_pair_stage_bytes(nt);
+    uint64_t* bars = (uint64_t*)(base + stages * stage_bytes);
+    volatile uint32_t* tmem_slot = (volatile uint32_t*)(bars + 2 * I8_PAIR_STAGES + 4);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    const uint32_t ring = smem_u32(base), full0 = smem_u32(bars), empty0 = smem_u32(bars + I8_PAIR_STAGES),
+                   acc_full0 = smem_u32(bars + 2 * I8_PAIR_STAGES), acc_empty0 = acc_full0 + 16;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)blockIdx.x & 1, first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full0 + 8 * a, 1); mbar_init(acc_empty0 + 8 * a, 16); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int st = 0, filled = 0;
+            uint32_t par = 0;
+            for (int t = first; t < tiles && !*abort_flag; t += step) {
+                const int32_t n0 = (t / t_tiles) * 2 * I8_TN + rank * I8_TN, m0 = (t % t_tiles) * nt + rank * (nt / 2);
+                for (int s = 0; s < slices; ++s) {
+                    if (filled == stages) {
+                        if (!mbar_wait_soon(empty0 + 8 * st, par ^ 1)) { *abort_flag = I8_ERR_EMPTY; break; }
+                    } else ++filled;
+                    const uint32_t dst = ring + st * stage_bytes, fb = cluster_addr(full0 + 8 * st, 0);
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * st, 2 * stage_bytes);
+                    if (KN) tma_load_2d_pair(dst, &map_w, n0, s * I8_KS, fb);
+                    else tma_load_2d_pair(dst, &map_w, s * I8_KS, n0, fb);
+                    tma_load_2d_pair(dst + I8_W_BYTES, &map_x, s * I8_KS, m0, fb);
+                    if (++st == stages) { st = 0; par ^= 1; }
+                }
+            }
+            // the last commits arrive here: stay until they have
+            const bool wrapped = filled == stages;
+            if (!wrapped) st = 0;
+            for (int i = 0; i < filled && !*abort_flag; ++i) {
+                if (!mbar_wait_soon(empty0 + 8 * st, wrapped ? par ^ 1 : 0)) *abort_flag = I8_ERR_EMPTY;
+                if (++st == stages) { st = 0; par ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int st = 0, acc = 0, used = 0;
+            uint32_t par = 0, acc_par = 0;
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (KN ? 1u << 15 : 0u) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(2 * I8_TN >> 4) << 24);
+            for (int t = first; t < tiles && !*abort_flag; t += step) {
+                if (used >= 2 && !mbar_wait_soon(acc_empty0 + 8 * acc, acc_par ^ 1)) { *abort_flag = I8_ERR_ACC; break; }
+                ++used;
+                tc_fence_after();
+                const uint32_t d = tmem + 256 * acc;
+                for (int s = 0; s < slices; ++s) {
+                    if (!mbar_wait_soon(full0 + 8 * st, par)) { *abort_flag = I8_ERR_FULL; break; }
+                    tc_fence_after();
+                    const uint32_t w = ring + st * stage_bytes, x = w + I8_W_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < I8_KS / 32; ++kk)
+                        umma_i8_pair(d, desc_sw128(w + kk * (KN ? 32 * 128 : 32)), desc_sw128(x + kk * 32), idesc, s > 0 || kk > 0);
+                    umma_commit_pair(empty0 + 8 * st);
+                    if (++st == stages) { st = 0; par ^= 1; }
+                }
+                umma_commit_pair(acc_full0 + 8 * acc);
+                if (++acc == 2) { acc = 0; acc_par ^= 1; }
+            }
+        }
+    } else {
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        int acc = 0;
+        uint32_t acc_par = 0;
+        for (int t = first; t < tiles; t += step) {
+            const int64_t ch = (int64_t)(t / t_tiles) * 2 * I8_TN + rank * I8_TN + 32 * quad + lane, m0 = (int64_t)(t % t_tiles) * nt;
+            const float sbv = sb && ch < n ? sb[ch] : 1.0f;
+            if (!mbar_wait_soon(acc_full0 + 8 * acc, acc_par)) { *abort_flag = I8_ERR_ACC; break; }
+            if (*abort_flag) break;
+            tc_fence_after();
+            const uint32_t from = tmem + 256 * acc + ((uint32_t)(32 * quad) << 16);
+            T* out = C + m0 * ldc + ch;
+            for (int q = half; q < nt / 16; q += 2) {
+                uint32_t r[16];
+                tmem_ld16(from + 16 * q, r);
+                const int64_t mine = m0 + 16 * q + (lane & 15);
+                const float sav = sa && mine < m ? sa[mine] : 1.0f;
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float a = __shfl_sync(~0u, sav, j);
+                    if (ch < n && m0 + 16 * q + j < m) out[(16 * q + j) * ldc] = Out<T>::make((int)r[j], a, sbv);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * acc, 0));
+            if (++acc == 2) { acc = 0; acc_par ^= 1; }
+        }
+    }
+    __syncwarp();
+    if (*abort_flag) {
+        if (lane == 0) atomicCAS(&g_i8_status, 0, (int)*abort_flag);
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    }
+    tc_fence_before();
+    cluster_sync();            // the other block's arrivals and the pair's products have ended
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
 // rows x len bytes, rows `pitch` bytes apart; box: 128 bytes x box_rows
 int make_map(CUtensorMap* map, const int8_t* ptr, int64_t rows, int64_t len, int64_t pitch, int box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();
@@ -182,15 +314,28 @@ struct Product {
     int64_t ldc, m, k, n;
 };
 
+// Shared memory beyond 48 KB is granted to a kernel once a device (`done`: a bit for each of the first 64; others every time).
+int grant_smem(const void* kernel, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    VI_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return VI_OK;
+    VI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I8_MAX_SMEM));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return VI_OK;
+}
+
 template <typename T, bool KN>
 int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
+    static std::atomic<uint64_t> granted{0};
     CUtensorMap map_w, map_x;
     int rc = KN ? make_map(&map_w, p.B, p.k, p.n, p.ldb, I8_KS) : make_map(&map_w, p.B, p.n, p.k, p.ldb, I8_TN);
     if (rc) return rc;
     rc = make_map(&map_x, p.A, p.m, p.k, p.lda, plan.nt);
     if (rc) return rc;
     const int smem = plan.stages * i8_stage_bytes(plan.nt) + 1024 + I8_TAIL;
-    VI_CUDA(cudaFuncSetAttribute(k_int8_umma<T, KN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    rc = grant_smem((const void*)k_int8_umma<T, KN>, granted);
+    if (rc) return rc;
     const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, n_tiles = (p.n + I8_TN - 1) / I8_TN;
     VI_REQUIRE(t_tiles * n_tiles * plan.split <= 0x7FFFFFFF, "int8_matmul: matrix too large for one launch");
     cudaLaunchConfig_t cfg = {};
@@ -213,8 +358,39 @@ int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
     return p.by_channel ? launch_umma<T, false>(p, plan, st) : launch_umma<T, true>(p, plan, st);
 }
 
+template <typename T, bool KN>
+int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
+    static std::atomic<uint64_t> granted{0};
+    CUtensorMap map_w, map_x;
+    int rc = KN ? make_map(&map_w, p.B, p.k, p.n, p.ldb, I8_KS) : make_map(&map_w, p.B, p.n, p.k, p.ldb, I8_TN);
+    if (rc) return rc;
+    rc = make_map(&map_x, p.A, p.m, p.k, p.lda, plan.nt / 2);
+    if (rc) return rc;
+    const int smem = plan.stages * i8_pair_stage_bytes(plan.nt) + 1024 + I8_PAIR_TAIL;
+    rc = grant_smem((const void*)k_int8_pair<T, KN>, granted);
+    if (rc) return rc;
+    const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, tiles = t_tiles * ((p.n + 2 * I8_TN - 1) / (2 * I8_TN));
+    VI_REQUIRE(tiles <= 0x3FFFFFFF, "int8_matmul: matrix too large for one launch");
+    k_int8_pair<T, KN><<<(unsigned)(2 * (tiles < 74 ? tiles : 74)), I8_PAIR_THREADS, smem, st>>>(
+        map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles, (int)tiles, (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.stages);
+    return vi::check_launch("k_int8_pair");
+}
+
+template <typename T>
+int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
+    if (!plan.pair) return launch_umma<T>(p, plan, st);
+    return p.by_channel ? launch_pair<T, false>(p, plan, st) : launch_pair<T, true>(p, plan, st);
+}
+
 Plan make_plan(int64_t m, int64_t k, int64_t n) {
     Plan p;
+    p.pair = m > 256 && n > 256;
+    if (p.pair) {
+        p.nt = 256;
+        p.split = 1;
+        p.stages = 200 * 1024 / i8_pair_stage_bytes(p.nt);
+        return p;
+    }
     p.nt = m >= 256 ? 256 : (int)((m + 15) / 16 * 16);
     const int64_t slices = (k + I8_KS - 1) / I8_KS, tiles = ((m + p.nt - 1) / p.nt) * ((n + I8_TN - 1) / I8_TN);
     p.split = 1;
@@ -300,11 +476,11 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     const Product p = {A, B, lda, ldb, nk, sa, sb, C, ldc, m, k, n};
     const Plan plan = make_plan(m, k, n);
     switch (out_type) {
-        case VI_F32: return launch_umma<float>(p, plan, st);
-        case VI_F16: return launch_umma<__half>(p, plan, st);
-        case VI_BF16: return launch_umma<__nv_bfloat16>(p, plan, st);
-        case VI_I32: return launch_umma<int32_t>(p, plan, st);
-        default: return launch_umma<uint64_t>(p, plan, st);
+        case VI_F32: return launch_product<float>(p, plan, st);
+        case VI_F16: return launch_product<__half>(p, plan, st);
+        case VI_BF16: return launch_product<__nv_bfloat16>(p, plan, st);
+        case VI_I32: return launch_product<int32_t>(p, plan, st);
+        default: return launch_product<uint64_t>(p, plan, st);
     }
 }
 

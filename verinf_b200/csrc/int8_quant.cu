@@ -148,7 +148,7 @@ extern "C" int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_
     VI_REQUIRE(scale && ((uintptr_t)scale) % 4 == 0, "int8_quantize_rows: null or misaligned scale");
     VI_REQUIRE(k == 0 || (x && q), "int8_quantize_rows: null pointer");
     VI_REQUIRE(((uintptr_t)x) % (dtype == VI_F32 ? 4 : 2) == 0, "int8_quantize_rows: x is not aligned to its type");
-    VI_REQUIRE(m == 1 || (x_stride >= k && q_stride >= k), "int8_quantize_rows: rows overlap (stride below k)");
+    VI_REQUIRE(m == 1 || (x_stride >= 0 && q_stride >= k), "int8_quantize_rows: negative distance of rows, or output rows that overlap");
     cudaStream_t st = (cudaStream_t)stream;
     if (m == 1) { x_stride = 0; q_stride = 0; }
     if (dtype == VI_F32) return launch<float>(x, m, k, x_stride, q, q_stride, scale, st);

@@ -17,23 +17,40 @@ from ._lib import LIB, check, on_device, raw_stream
 # element types of the C ABI (enum in include/verinf_b200.h)
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: 3, torch.uint64: 4}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_INT8 = (torch.int8,)
 MAX_K = 131071        # int8 products that a 32-bit sum holds
 
 
-def _matrix(t, what, name, dtypes):
+def matrix(t, what, name, dtypes):
+    """(rows, columns, elements from a row to the next) of a 2-D CUDA tensor whose rows' entries lie together."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{what}: {name} must be a CUDA tensor")
     if t.dtype not in dtypes:
         raise RuntimeError(f"{what}: {name} has dtype {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise RuntimeError(f"{what}: {name} must be 2-D")
+    rows, cols = shape
+    apart, step = t.stride()
+    if step != 1 and cols > 1:
+        raise RuntimeError(f"{what}: the entries of a row of {name} must lie together (stride {step})")
+    return rows, cols, apart if rows > 1 else cols
 
 
-def _rows_apart(t, what, name):
-    """Elements from a row of a 2-D tensor to the next; the entries of a row must lie together."""
-    if t.size(1) > 1 and t.stride(1) != 1:
-        raise RuntimeError(f"{what}: the entries of a row of {name} must lie together (stride {t.stride(1)})")
-    return t.stride(0) if t.size(0) > 1 else max(t.size(1), 1)
+def _output(out, shape, dev, what, name, dtypes):
+    """Row distance of a tensor to be written."""
+    rows, cols, apart = matrix(out, what, name, dtypes)
+    if (rows, cols) != shape or out.device != dev:
+        raise RuntimeError(f"{what}: {name} must be {shape[0]} x {shape[1]} on the inputs' device")
+    if apart < cols:
+        raise RuntimeError(f"{what}: rows of {name} overlap")
+    return apart
+
+
+def _vector(s, n, dev, what, name):
+    if not isinstance(s, torch.Tensor) or s.dtype is not torch.float32 or s.device != dev or s.shape != (n,) or not s.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be a contiguous fp32 tensor of {n} scales on the inputs' device")
+    return s.data_ptr()
 
 
 def int8_quantize_rows(x, out=None):
@@ -44,38 +61,43 @@ def int8_quantize_rows(x, out=None):
     that holds a NaN or an infinity has scale NaN and zeros.  `out`: a pair (q, scale) to write into; the rows of q may be any
     distance apart."""
     what = "int8_quantize_rows"
-    _matrix(x, what, "x", _FLOATS)
-    m, k = x.shape
-    xs = _rows_apart(x, what, "x")
-    if xs < k:
-        x, xs = x.contiguous(), k                       # expanded rows
+    m, k, xs = matrix(x, what, "x", _FLOATS)
+    dev = x.device
     if out is None:
-        q = torch.empty((m, k), dtype=torch.int8, device=x.device)
-        scale = torch.empty((m,), dtype=torch.float32, device=x.device)
-        qs = k
+        q, qs = x.new_empty((m, k), dtype=torch.int8), k
+        scale = x.new_empty(m, dtype=torch.float32)
+        scale_ptr = scale.data_ptr()
     else:
         q, scale = out
-        _matrix(q, what, "out[0]", (torch.int8,))
-        if q.shape != x.shape or q.device != x.device:
-            raise RuntimeError(f"{what}: out[0] must have x's shape and device")
-        qs = _rows_apart(q, what, "out[0]")
-        if qs < k:
-            raise RuntimeError(f"{what}: rows of out[0] overlap")
-        if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.shape != (m,) or \
-                scale.device != x.device or not scale.is_contiguous():
-            raise RuntimeError(f"{what}: out[1] must be a contiguous fp32 tensor of {m} scales on x's device")
-    with on_device(x.device):
-        check(LIB.vi_int8_quantize_rows(x.data_ptr(), DTYPE_CODES[x.dtype], m, k, xs, q.data_ptr(), qs, scale.data_ptr(),
-                                        raw_stream(x.device)))
+        qs = _output(q, (m, k), dev, what, "out[0]", _INT8)
+        scale_ptr = _vector(scale, m, dev, what, "out[1]")
+    index = dev.index
+    with on_device(index):
+        rc = LIB.vi_int8_quantize_rows(x.data_ptr(), DTYPE_CODES[x.dtype], m, k, xs, q.data_ptr(), qs, scale_ptr, raw_stream(index))
+    if rc:
+        check(rc)
     return q, scale
 
 
-def _scales(s, n, dev, what, name):
-    if s is None:
-        return None
-    if not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or s.device != dev or s.shape != (n,) or not s.is_contiguous():
-        raise RuntimeError(f"{what}: {name} must be a contiguous fp32 tensor of {n} scales on the operands' device")
-    return s.data_ptr()
+def _weight(B, what):
+    """(k, n, by channel or not, distance of rows or channels) of a (k, n) operand that lies either way, copied if it is
+    expanded."""
+    if not isinstance(B, torch.Tensor) or not B.is_cuda:
+        raise RuntimeError(f"{what}: B must be a CUDA tensor")
+    if B.dtype is not torch.int8:
+        raise RuntimeError(f"{what}: B has dtype {B.dtype}, expected torch.int8")
+    shape = B.shape
+    if len(shape) != 2:
+        raise RuntimeError(f"{what}: B must be 2-D")
+    k, n = shape
+    s0, s1 = B.stride()
+    if (s1 == 1 or n == 1) and (s0 >= n or k == 1):
+        return B, k, n, 0, s0 if k > 1 else n
+    if (s0 == 1 or k == 1) and (s1 >= k or n == 1):
+        return B, k, n, 1, s1 if n > 1 else k
+    if s0 and s1:
+        raise RuntimeError(f"{what}: the rows or the columns of B must lie together (strides {B.stride()})")
+    return B.contiguous(), k, n, 0, n
 
 
 def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
@@ -90,51 +112,38 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
     boundaries are read in place; others are copied on every call.  `out`: a tensor of `dtype` to write into, rows any
     distance apart; it must not share memory with the operands."""
     what = "int8_matmul"
-    _matrix(A, what, "A", (torch.int8,))
-    _matrix(B, what, "B", (torch.int8,))
-    if A.size(1) != B.size(0):
+    m, k, lda = matrix(A, what, "A", _INT8)
+    B, kb, n, by_channel, ldb = _weight(B, what)
+    dev = A.device
+    if k != kb:
         raise RuntimeError(f"{what}: inner dim mismatch")
-    if A.device != B.device:
+    if B.device != dev:
         raise RuntimeError(f"{what}: operands on different devices")
-    if dtype not in DTYPE_CODES:
+    code = DTYPE_CODES.get(dtype)
+    if code is None:
         raise RuntimeError(f"{what}: dtype must be float32, float16, bfloat16, int32 or uint64")
-    m, k = A.shape
-    n = B.size(1)
     if k > MAX_K:
         raise RuntimeError(f"{what}: k = {k}, but 32-bit sums hold at most {MAX_K} products")
-    if dtype not in _FLOATS and (scale_a is not None or scale_b is not None):
+    if code > 2 and (scale_a is not None or scale_b is not None):
         raise RuntimeError(f"{what}: whole-number outputs take no scales")
-    dev = A.device
-    lda = _rows_apart(A, what, "A")
-    if (B.stride(1) == 1 or n == 1) and (B.stride(0) >= n or k == 1):
-        by_channel, ldb = 0, (B.stride(0) if k > 1 else n)
-    elif (B.stride(0) == 1 or k == 1) and (B.stride(1) >= k or n == 1):
-        by_channel, ldb = 1, (B.stride(1) if n > 1 else k)
-    elif B.stride(0) and B.stride(1):
-        raise RuntimeError(f"{what}: the rows or the columns of B must lie together (strides {B.stride()})")
-    else:
-        B = B.contiguous()                              # expanded
-        by_channel, ldb = 0, n
     if lda < k:
-        A, lda = A.contiguous(), k
-    sa, sb = _scales(scale_a, m, dev, what, "scale_a"), _scales(scale_b, n, dev, what, "scale_b")
+        A, lda = A.contiguous(), k                      # expanded
+    sa = None if scale_a is None else _vector(scale_a, m, dev, what, "scale_a")
+    sb = None if scale_b is None else _vector(scale_b, n, dev, what, "scale_b")
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=dev)
-        ldc = n
+        out, ldc = A.new_empty((m, n), dtype=dtype), n
     else:
-        _matrix(out, what, "out", (dtype,))
-        if out.shape != (m, n) or out.device != dev:
-            raise RuntimeError(f"{what}: out must be ({m}, {n}) on the operands' device")
-        ldc = _rows_apart(out, what, "out")
-        if ldc < n:
-            raise RuntimeError(f"{what}: rows of out overlap")
-    a, b = A.data_ptr(), B.data_ptr()
-    room, nb = None, LIB.vi_int8_matmul_scratch_bytes(a, lda, b, ldb, by_channel, m, k, n)
-    if nb:
-        room = torch.empty((nb,), dtype=torch.int8, device=dev)      # of the current stream: calls on two streams share nothing
-    with on_device(dev):
-        check(LIB.vi_int8_matmul(a, lda, b, ldb, by_channel, sa, sb, out.data_ptr(), DTYPE_CODES[dtype], ldc, m, k, n,
-                                 room.data_ptr() if nb else None, nb, raw_stream(dev)))
+        ldc = _output(out, (m, n), dev, what, "out", (dtype,))
+    index = dev.index
+    a, b, room, nb = A.data_ptr(), B.data_ptr(), None, 0
+    if (a | b | lda | ldb) & 15:                        # an operand may have to be copied
+        nb = LIB.vi_int8_matmul_scratch_bytes(a, lda, b, ldb, by_channel, m, k, n)
+        room = A.new_empty(nb)                          # of the current stream: calls on two streams share nothing
+    with on_device(index):
+        rc = LIB.vi_int8_matmul(a, lda, b, ldb, by_channel, sa, sb, out.data_ptr(), code, ldc, m, k, n,
+                                room.data_ptr() if nb else None, nb, raw_stream(index))
+    if rc:
+        check(rc)
     return out
 
 
