@@ -356,7 +356,7 @@ int vi_int8_matmul_status(int* code);
  * nothing but -inf has logprob -inf and entropy 0; one that holds a NaN or +inf has NaN in all its numbers and an empty
  * list.  1e-6 <= temperature <= 1e6. */
 int vi_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
-                      const int64_t* tokens, int top, float temperature,
+                      const int64_t* tokens, int top, double temperature,
                       float* logprob, float* entropy, float* top_logprob, int64_t* top_token, void* stream);
 
 /* ---- per-kernel timing ------------------------------------------------------------

@@ -79,7 +79,7 @@ SIGNATURES = {
     "vi_int8_matmul_scratch_bytes": (_i64, [_p, _i64, _p, _i64, _int, _i64, _i64, _i64]),
     "vi_int8_matmul": (_int, [_p, _i64, _p, _i64, _int, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "vi_int8_matmul_status": (_int, [C.POINTER(_int)]),
-    "vi_token_logprobs": (_int, [_p, _int, _i64, _i64, _i64, _p, _int, C.c_float, _p, _p, _p, _p, _p]),
+    "vi_token_logprobs": (_int, [_p, _int, _i64, _i64, _i64, _p, _int, _dbl, _p, _p, _p, _p, _p]),
     "vi_profile_enable": (None, [_int]),
     "vi_profile_num_tags": (_int, []),
     "vi_profile_tag_name": (C.c_char_p, [_int]),
