@@ -160,6 +160,25 @@ def test_quantize_borders(i8, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 7), (torch.float16, 10)])
+@pytest.mark.parametrize("gap", [0, 1, 2, 4, 7])
+def test_quantize_every_quotient_of_16_bits(i8, dtype, bits, gap):
+    """Rows with every significand as their maximum, in them every significand `gap` binades lower, against whole numbers:
+    127 x / a = 127 i 2^-gap / j for significands i and j.  fp16 values near 1, so that none is subnormal."""
+    n = 1 << bits
+    j = torch.arange(n, 2 * n, device="cuda")
+    i = torch.arange(n, 2 * n, device="cuda").repeat(n, 1)
+    i = torch.where(i <= j[:, None] << gap, i, 0)                    # not above the maximum
+    x = torch.cat([i * 2.0 ** (-gap - bits), -(j[:, None] * 2.0 ** -bits)], 1)
+    q, _ = i8.int8_quantize_rows(x.to(dtype))
+    num, den = 127 * i, j[:, None] << gap
+    low, rest = num // den, num % den * 2
+    want = low + ((rest > den) | ((rest == den) & (low % 2 == 1)))
+    assert (x.to(dtype).double() == x).all()
+    assert torch.equal(q[:, :-1].long(), want) and (q[:, -1] == -127).all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_quantize_extremes(i8, dtype):
     """The type's largest, smallest and subnormal values, rows of zeros, rows with NaN and infinities."""

@@ -18,9 +18,13 @@
 
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
+#include "f32x2.cuh"
+#include "packs.cuh"
 #include "umma.cuh"
 
 namespace {
+
+using namespace vf2;
 
 constexpr int LP_MAX_TOP = 32, LP_GROUPS = 64, LP_CANDIDATES = 1024, LP_UNROLL = 4, LP_MAX_SPLIT = 8;
 constexpr float LP_LOW = -3.402823466e38f;       // least finite value: a maximum starts here, so that -inf - max is -inf and not NaN
@@ -46,24 +50,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {       // NaN if eit
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// two fp32 operations an instruction
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // The entries of a 16-byte load: two at a time as fp32, the largest of them, -inf replaced by LP_CLAMP on demand.
 template <typename T> struct Entries;
 template <> struct Entries<float> {
@@ -124,27 +110,6 @@ template <> struct Entries<__nv_bfloat16> {
     static __device__ __forceinline__ float clamp_one(float v) { return v; }
 };
 
-// A pack that the row shares with what lies before or behind it: the row's entries, -inf in the other places.
-template <typename T>
-__device__ __noinline__ uint4 edge_pack(const T* x, int64_t first, int64_t vocab) {
-    using R = typename Entries<T>::Raw;
-    constexpr int N = Entries<T>::N, IN_WORD = N / 4;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = Entries<T>::NOTHING;
-#pragma unroll
-        for (int e = 0; e < IN_WORD; ++e) {
-            const int64_t at = first + i * IN_WORD + e;
-            if (at >= 0 && at < vocab) {
-                const uint32_t keep = IN_WORD == 1 ? 0u : e ? 0x0000FFFFu : 0xFFFF0000u;
-                w[i] = (w[i] & keep) | (uint32_t)reinterpret_cast<const R*>(x)[at] << (16 * e);
-            }
-        }
-    }
-    return {w[0], w[1], w[2], w[3]};
-}
-
 struct Stat { float m, s, w; };      // max, sum 2^a, sum 2^a a
 
 // a of an entry against a maximum.  Short form: x c - m c with one rounded m c, the same for all entries of a maximum, so that
@@ -199,11 +164,8 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
     const int rank = (int)blockIdx.x % split;
     const int64_t row = blockIdx.x / (unsigned)split;
     const T* x = logits + row * stride;
-    // packs on the 16-byte grid: pack p holds the entries p N - head .. p N - head + N - 1 that the row has
-    const int head = (int)(((uintptr_t)x & 15) / sizeof(T));
-    const uint4* packs = reinterpret_cast<const uint4*>((uintptr_t)x & ~(uintptr_t)15);
-    const int64_t npack = (vocab + head + N - 1) / N, p0 = npack * rank / split, p1 = npack * (rank + 1) / split;
-    const int64_t whole0 = head ? 1 : 0, whole1 = (vocab + head) / N;            // packs of the row alone: [whole0, whole1)
+    const vpk::Row<typename E::Raw> packs(x, vocab);
+    const int64_t p0 = packs.count * rank / split, p1 = packs.count * (rank + 1) / split;
 
     Stat st = {LP_LOW, 0.0f, 0.0f};
     // The packs of a thread fall into LP_UNROLL shares: the largest entry of each, and the first pack that reached it.
@@ -211,21 +173,27 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
     uint32_t mine_pack[LP_UNROLL];
 #pragma unroll
     for (int u = 0; u < LP_UNROLL; ++u) { mine[u] = -CUDART_INF_F; mine_pack[u] = 0; }
-    const int64_t inner1 = p1 < whole1 ? p1 : whole1;
-    for (int64_t base = p0 + tid; base < p1; base += LP_UNROLL * NT) {
-        uint4 q[LP_UNROLL];
-        if (base >= whole0 && base + (LP_UNROLL - 1) * NT < inner1) {
+    const int64_t inner1 = p1 < packs.whole1 ? p1 : packs.whole1;
+    auto fetch = [&](uint4 (&q)[LP_UNROLL], int64_t base) {
+        if (base >= packs.whole0 && base + (LP_UNROLL - 1) * NT < inner1) {
 #pragma unroll
-            for (int u = 0; u < LP_UNROLL; ++u) q[u] = __ldg(packs + base + u * NT);
+            for (int u = 0; u < LP_UNROLL; ++u) q[u] = __ldg(packs.packs + base + u * NT);
         } else {                                  // packs beyond the share count as -inf
 #pragma unroll
             for (int u = 0; u < LP_UNROLL; ++u) {
                 const int64_t p = base + u * NT;
                 q[u] = {E::NOTHING, E::NOTHING, E::NOTHING, E::NOTHING};
-                if (p >= whole0 && p < inner1) q[u] = __ldg(packs + p);
-                else if (p < p1) q[u] = edge_pack(x, p * N - head, vocab);
+                if (p < p1) q[u] = packs.load(p, E::NOTHING);
             }
         }
+    };
+    uint4 next[LP_UNROLL];
+    fetch(next, p0 + tid);
+    for (int64_t base = p0 + tid; base < p1; base += LP_UNROLL * NT) {
+        uint4 q[LP_UNROLL];
+#pragma unroll
+        for (int u = 0; u < LP_UNROLL; ++u) q[u] = next[u];
+        if (base + LP_UNROLL * NT < p1) fetch(next, base + LP_UNROLL * NT);
         float most = st.m;
 #pragma unroll
         for (int u = 0; u < LP_UNROLL; ++u) {
@@ -299,7 +267,7 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
             const uint64_t b = __shfl_xor_sync(~0u, k, o);
             k = b > k ? b : k;
         }
-        if (tid % IN_GROUP == 0) group[tid / IN_GROUP] = k;
+        if (tid % IN_GROUP == 0) group[tid / IN_GROUP] = k ? k : (uint64_t)(tid / IN_GROUP);      // distinct, and below every key
     }
     if (tid == 0) { n_cand = 0; n_flag = 0; }
     if (tid < LP_MAX_TOP) best[tid] = 0;
@@ -315,20 +283,19 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
         }
         if (lane == 0) total = t;
     }
-    if (top && tid >= NT - LP_GROUPS) {          // rank among the groups; those without a key count by their number
-        const int g = tid - (NT - LP_GROUPS);
-        const uint64_t k = group[g];
+    if (top && tid >= NT - LP_GROUPS) {          // rank among the groups
+        const uint64_t k = group[tid - (NT - LP_GROUPS)];
         int above = 0;
 #pragma unroll 8
         for (int i = 0; i < LP_GROUPS; i += 2) {
             const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&group[i]);
-            above += (o.x > k || (o.x == k && i < g)) + (o.y > k || (o.y == k && i + 1 < g));
+            above += (o.x > k) + (o.y > k);
         }
         if (above == top - 1) limit = k;
     }
     __syncthreads();
     if (top) {
-        const uint64_t lim = limit;
+        const uint64_t lim = limit < LP_GROUPS ? 0 : limit;       // fewer groups than `top` have a key: every entry counts
         const float lim_value = lim ? unordered((uint32_t)(lim >> 32)) : LP_LOW;
         unsigned vote[LP_UNROLL];                 // shares that may hold some of the best
         int votes = 0;
@@ -349,25 +316,27 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
         }
         __syncthreads();
         const unsigned per = (unsigned)((p1 - p0 + LP_UNROLL * NT - 1) / (LP_UNROLL * NT));
-        const int64_t items = (int64_t)n_flag * per;
-        for (int64_t item = tid; item < items; item += NT) {               // their packs, one a thread
-            const unsigned f = (unsigned)((uint64_t)item / per), j = (unsigned)item - f * per;
+        const unsigned items = (unsigned)n_flag * per;                     // at most 4 NT shares of 2^31 / (4 NT) packs
+        for (unsigned item = tid; item < items; item += NT) {              // their packs, one a thread
+            const unsigned f = item / per, j = item - f * per;
             const int64_t p = p0 + flagged[f] + (int64_t)j * (LP_UNROLL * NT);
             if (p >= p1) continue;
-            const uint4 q = p >= whole0 && p < whole1 ? __ldg(packs + p) : edge_pack(x, p * N - head, vocab);
+            const uint4 q = packs.load(p, E::NOTHING);
             if (!(E::largest(q) >= lim_value)) continue;
-            const int first = (int)(p * N - head);
+            unsigned hits = 0;
 #pragma unroll
             for (int i = 0; i < N / 2; ++i) {
-                float v[2];
-                E::two(q, i, v[0], v[1]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    // the same order as that of the group keys: value, then pack
-                    if (v[e] >= lim_value && make_key(v[e], (uint32_t)p) >= lim) {
-                        const int at = atomicAdd(&n_cand, 1);
-                        if (at < LP_CANDIDATES) cand[at] = make_key(v[e], (uint32_t)(first + 2 * i + e));
-                    }
+                float v0, v1;
+                E::two(q, i, v0, v1);
+                hits |= (v0 >= lim_value ? 1u << (2 * i) : 0u) | (v1 >= lim_value ? 2u << (2 * i) : 0u);
+            }
+            while (hits) {
+                const int64_t i = packs.first(p) + __ffs(hits) - 1;
+                hits &= hits - 1;
+                const float v = E::one(x + i);
+                if (make_key(v, (uint32_t)p) >= lim) {                     // the same order as that of the group keys: value, then pack
+                    const int at = atomicAdd(&n_cand, 1);
+                    if (at < LP_CANDIDATES) cand[at] = make_key(v, (uint32_t)i);
                 }
             }
         }
@@ -387,7 +356,7 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
             }
         } else {
             // Shares made so that a few threads hold most of the large entries: one pass over the share for each alternative.
-            const int64_t i0 = p0 * N - head < 0 ? 0 : p0 * N - head, i1 = p1 * N - head < vocab ? p1 * N - head : vocab;
+            const int64_t i0 = packs.first(p0) < 0 ? 0 : packs.first(p0), i1 = packs.first(p1) < vocab ? packs.first(p1) : vocab;
             uint64_t below = ~0ull;
             for (int j = 0; j < top && below; ++j) {
                 uint64_t k = 0;
@@ -497,9 +466,15 @@ int launch(const void* logits, int64_t rows, int64_t vocab, int64_t stride, cons
     return go(logits, rows, vocab, stride, tokens, top, c, inv_t, logprob, entropy, top_logprob, top_token, plan.split, st);
 }
 
+// Many rows: small blocks, whose ends (sums, list) hide behind other blocks' loads; 128 threads, for rows of up to 1024 packs
+// 64 (us with 64 / 128 / 256 threads and 20 alternatives: 4096 x 32000 bf16 87 / 61 / 71, 4096 x 4000 20 / 24 / 42, 1000 x
+// 32000 24 / 19 / 22).  Few rows: 256 threads, and while that gives no more than two blocks an SM, long rows go to clusters,
+// down to 2000 packs a block (1 x 32000 fp32 on 1 / 2 / 4 / 8 blocks 7.6 / 7.2 / 6.8 / 7.2, 8 x 128000 bf16 14 / 11 / 8.7 /
+// 8.3, 64 x 202048 fp16 23 / 17 / 14 / 16, 300 x 32000 bf16 11 / 16 / 22).
 Plan make_plan(int64_t rows, int64_t packs) {
+    if (rows >= 512) return {packs <= 1024 ? 64 : 128, 1};
     Plan p = {256, 1};
-    while (p.split < LP_MAX_SPLIT && rows * p.split < 4 * 148 && packs >= p.split * 4 * 256) p.split *= 2;
+    while (p.split < LP_MAX_SPLIT && rows * p.split * 2 <= 2 * 148 && packs > p.split * 4000) p.split *= 2;
     return p;
 }
 
