@@ -10,6 +10,7 @@
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
 #include "gl.cuh"
+#include "launch.cuh"
 #include "umma.cuh"
 
 namespace {
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    vi::await_inputs();
     for (int j = tid; j < nt; j += I8_THREADS) sa_s[j] = sa && m0 + j < m ? sa[m0 + j] : 1.0f;
     tc_fence_before();
     __syncthreads();
@@ -118,6 +120,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     }
     __syncwarp();
     bool ok = mbar_wait_soon(accb, 0);
+    vi::release_next();
     if (!ok && *abort_flag == 0) *abort_flag = I8_ERR_ACC;
     tc_fence_after();
     ok = ok && *abort_flag == 0;
@@ -171,7 +174,7 @@ constexpr int I8_PAIR_TAIL = (2 * I8_PAIR_STAGES + 4 + 1) * 8 + 24;
 __host__ __device__ inline int i8_pair_stage_bytes(int nt) { return I8_W_BYTES + nt / 2 * I8_KS; }
 
 template <typename T, bool KN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_PAIR_THREADS)
+__global__ void __launch_bounds__(I8_PAIR_THREADS)
 k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ sa,
             const float* __restrict__ sb, T* __restrict__ C, int64_t ldc, int64_t m, int64_t n, int t_tiles, int tiles, int slices, int nt, int stages) {
     extern __shared__ uint8_t i8_raw[];
@@ -195,6 +198,7 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
+    vi::await_inputs();
     tc_fence_before();
     __syncthreads();
     cluster_sync();
@@ -282,6 +286,7 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         }
     }
     __syncwarp();
+    vi::release_next();
     if (*abort_flag) {
         if (lane == 0) atomicCAS(&g_i8_status, 0, (int)*abort_flag);
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);
@@ -338,19 +343,9 @@ int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
     if (rc) return rc;
     const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, n_tiles = (p.n + I8_TN - 1) / I8_TN;
     VI_REQUIRE(t_tiles * n_tiles * plan.split <= 0x7FFFFFFF, "int8_matmul: matrix too large for one launch");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(t_tiles * n_tiles * plan.split));
-    cfg.blockDim = dim3(I8_THREADS);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {(unsigned)plan.split, 1, 1};
-    cfg.attrs = attr;
-    cfg.numAttrs = plan.split > 1 ? 1 : 0;
-    VI_CUDA(cudaLaunchKernelEx(&cfg, k_int8_umma<T, KN>, map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles,
-                               (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.split, plan.stages));
-    return VI_OK;
+    return vi::launch_early("k_int8_umma", k_int8_umma<T, KN>, dim3((unsigned)(t_tiles * n_tiles * plan.split)), dim3(I8_THREADS), (size_t)smem, plan.split, st,
+                            map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles, (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.split,
+                            plan.stages);
 }
 
 template <typename T>
@@ -371,9 +366,9 @@ int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
     if (rc) return rc;
     const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, tiles = t_tiles * ((p.n + 2 * I8_TN - 1) / (2 * I8_TN));
     VI_REQUIRE(tiles <= 0x3FFFFFFF, "int8_matmul: matrix too large for one launch");
-    k_int8_pair<T, KN><<<(unsigned)(2 * (tiles < 74 ? tiles : 74)), I8_PAIR_THREADS, smem, st>>>(
-        map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles, (int)tiles, (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.stages);
-    return vi::check_launch("k_int8_pair");
+    return vi::launch_early("k_int8_pair", k_int8_pair<T, KN>, dim3((unsigned)(2 * (tiles < 74 ? tiles : 74))), dim3(I8_PAIR_THREADS), (size_t)smem, 2, st,
+                            map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles, (int)tiles, (int)((p.k + I8_KS - 1) / I8_KS), plan.nt,
+                            plan.stages);
 }
 
 template <typename T>
@@ -401,33 +396,64 @@ Plan make_plan(int64_t m, int64_t k, int64_t n) {
 }
 
 // ---- operands that TMA cannot read in place -----------------------------------------------------------------------
-// Rows that start off the 16-byte grid are copied to rows that start on it (a pass over those bytes; the caller's rows are
-// copied anew on every call).
-__global__ void __launch_bounds__(256) k_int8_align(const int8_t* __restrict__ src, int64_t pitch, int64_t rows, int64_t len, int8_t* __restrict__ dst, int64_t dst_pitch) {
-    const int64_t per = dst_pitch / 4, total = rows * per;
+// Rows that start off the 16-byte grid are copied to rows that start on it: a pass over those bytes, on every call (11008 rows
+// of 4096 bytes: see below).  A thread makes 16 bytes of the copy from the two grid cells that hold them, of which it reads only
+// those that hold bytes of the row.
+inline __host__ __device__ int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
+
+struct Rows {
+    const int8_t* src;
+    int8_t* dst;
+    int64_t pitch, rows, len;
+};
+
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int by) {      // 16 of 32 bytes, from `by` on
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (by & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
+    if (by & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
+    const int bits = 8 * (by & 3);
+    return {__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits)};
+}
+
+__global__ void __launch_bounds__(256) k_int8_align(const Rows first, const Rows second) {
+    vi::await_inputs();
+    const bool is_second = blockIdx.y == 1;
+    const Rows r = is_second ? second : first;
+    const int64_t per = up16(r.len) / 16, total = r.rows * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per, c = (i % per) * 4;
-        uint32_t v = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < len) v |= (uint32_t)(uint8_t)src[r * pitch + c + e] << (8 * e);
-        *(uint32_t*)(dst + r * dst_pitch + c) = v;
+        const int64_t row = i / per, c = (i - row * per) * 16;
+        const uintptr_t at = (uintptr_t)(r.src + row * r.pitch + c), end = at - c + r.len;
+        const uint4* cell = (const uint4*)(at & ~(uintptr_t)15);
+        const uint4 none = {0, 0, 0, 0};
+        const uint4 a = __ldg(cell), b = (uintptr_t)(cell + 1) < end && (at & 15) ? __ldg(cell + 1) : none;
+        reinterpret_cast<uint4*>(r.dst)[i] = shifted(a, b, (int)(at & 15));
     }
 }
 
-inline int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 inline bool in_place(const void* p, int64_t pitch) { return ((uintptr_t)p) % 16 == 0 && pitch % 16 == 0; }
 inline int64_t b_rows(int64_t k, int64_t n, bool by_channel) { return by_channel ? n : k; }
 inline int64_t b_len(int64_t k, int64_t n, bool by_channel) { return by_channel ? k : n; }
 
-int align_rows(const int8_t*& ptr, int64_t& pitch, int64_t rows, int64_t len, int8_t*& room, cudaStream_t st) {
-    if (in_place(ptr, pitch)) return VI_OK;
-    const int64_t to = up16(len), words = rows * (to / 4), want = (words + 255) / 256;
-    k_int8_align<<<(unsigned)(want < 148 * 16 ? want : 148 * 16), 256, 0, st>>>(ptr, pitch, rows, len, room, to);
-    ptr = room;
-    pitch = to;
-    room += rows * to;
-    return vi::check_launch("k_int8_align");
+// Copies those of the operands that need it to `room` and points p at the copies.
+int align_rows(Product& p, int8_t* room, cudaStream_t st) {
+    Rows todo[2];
+    int n = 0;
+    if (!in_place(p.A, p.lda)) {
+        todo[n++] = {p.A, room, p.lda, p.m, p.k};
+        p.A = room;
+        p.lda = up16(p.k);
+        room += p.m * p.lda;
+    }
+    if (!in_place(p.B, p.ldb)) {
+        const int64_t rows = b_rows(p.k, p.n, p.by_channel), len = b_len(p.k, p.n, p.by_channel);
+        todo[n++] = {p.B, room, p.ldb, rows, len};
+        p.B = room;
+        p.ldb = up16(len);
+    }
+    if (n == 0) return VI_OK;
+    const int64_t cells0 = todo[0].rows * (up16(todo[0].len) / 16), cells1 = n > 1 ? todo[1].rows * (up16(todo[1].len) / 16) : 0;
+    const int64_t want = ((cells0 > cells1 ? cells0 : cells1) + 255) / 256;
+    return vi::launch_early("k_int8_align", k_int8_align, dim3((unsigned)(want < 148 * 32 ? want : 148 * 32), (unsigned)n), dim3(256), 0, 1, st, todo[0], todo[n - 1]);
 }
 
 }  // namespace
@@ -468,12 +494,9 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     if (need && (scratch == nullptr || scratch_bytes < need))
         return vi::fail(VI_ERR_SCRATCH, "int8_matmul: scratch of at least %lld bytes required (see vi_int8_matmul_scratch_bytes)", (long long)need);
     VI_REQUIRE(!need || ((uintptr_t)scratch) % 16 == 0, "int8_matmul: scratch must be 16-byte aligned");
-    int8_t* room = (int8_t*)scratch;
-    int rc = align_rows(A, lda, m, k, room, st);
+    Product p = {A, B, lda, ldb, nk, sa, sb, C, ldc, m, k, n};
+    const int rc = align_rows(p, (int8_t*)scratch, st);
     if (rc) return rc;
-    rc = align_rows(B, ldb, b_rows(k, n, nk), b_len(k, n, nk), room, st);
-    if (rc) return rc;
-    const Product p = {A, B, lda, ldb, nk, sa, sb, C, ldc, m, k, n};
     const Plan plan = make_plan(m, k, n);
     switch (out_type) {
         case VI_F32: return launch_product<float>(p, plan, st);

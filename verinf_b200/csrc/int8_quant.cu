@@ -13,6 +13,7 @@
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "launch.cuh"
 #include "packs.cuh"
 
 namespace {
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const T* __restrict__ x,
     constexpr int N = 16 / (int)sizeof(T);
     __shared__ uint32_t part[32];
     const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    vi::await_inputs();
     if (r >= m) return;
     const vpk::Row<typename E::Raw> row(x + r * x_stride, k);
     int8_t* qr = q + r * q_stride;
@@ -200,6 +202,7 @@ __global__ void __launch_bounds__(1024) k_int8_quantize(const T* __restrict__ x,
         for (int j = 0; j < QT_KEEP; ++j) amax = max(amax, E::largest(keep[j]));
         for (int64_t i = tid + QT_KEEP * nt; i < row.count; i += nt) amax = max(amax, E::largest(row.load(i, 0)));
     }
+    vi::release_next();
     amax = __reduce_max_sync(0xFFFFFFFFu, amax);
     if (nt > 32) {
         if ((tid & 31) == 0) part[tid >> 5] = amax;
@@ -256,9 +259,8 @@ int launch(const void* x, int64_t m, int64_t k, int64_t x_stride, int8_t* q, int
     const unsigned nt = want <= 32 ? 32 : want >= 1024 ? 1024 : (unsigned)(want + 31) / 32 * 32;
     const unsigned rows = nt == 32 ? 8 : 1;
     const bool aligned = ((uintptr_t)x) % 16 == 0 && x_stride % N == 0 && ((uintptr_t)q) % N == 0 && q_stride % N == 0;
-    (aligned ? k_int8_quantize<T, true> : k_int8_quantize<T, false>)<<<(unsigned)((m + rows - 1) / rows), dim3(nt, rows), 0, st>>>(
-        (const T*)x, x_stride, m, k, q, q_stride, scale);
-    return vi::check_launch("k_int8_quantize");
+    return vi::launch_early("k_int8_quantize", aligned ? k_int8_quantize<T, true> : k_int8_quantize<T, false>, dim3((unsigned)((m + rows - 1) / rows)),
+                            dim3(nt, rows), 0, 1, st, (const T*)x, x_stride, m, k, q, q_stride, scale);
 }
 
 }  // namespace

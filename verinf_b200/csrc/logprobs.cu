@@ -19,6 +19,7 @@
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "launch.cuh"
 #include "packs.cuh"
 #include "umma.cuh"
 
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
     const int rank = (int)blockIdx.x % split;
     const int64_t row = blockIdx.x / (unsigned)split;
     const T* x = logits + row * stride;
+    vi::await_inputs();
     const vpk::Row<typename E::Raw> packs(x, vocab);
     const int64_t p0 = packs.count * rank / split, p1 = packs.count * (rank + 1) / split;
 
@@ -244,6 +246,7 @@ __global__ void __launch_bounds__(NT) k_token_logprobs(const T* __restrict__ log
             }
         }
     }
+    vi::release_next();
     // the warp's sums against the warp's maximum
     {
         const float m = unordered(__reduce_max_sync(~0u, ordered(st.m)));
@@ -446,17 +449,8 @@ struct Plan { int threads, split; };      // split <= threads / 32
 template <typename T, int NT>
 int launch(const void* logits, int64_t rows, int64_t vocab, int64_t stride, const int64_t* tokens, int top, float c, float inv_t, float* logprob,
            float* entropy, float* top_logprob, int64_t* top_token, int split, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * split));
-    cfg.blockDim = dim3(NT);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {(unsigned)split, 1, 1};
-    cfg.attrs = attr;
-    cfg.numAttrs = split > 1 ? 1 : 0;
-    VI_CUDA(cudaLaunchKernelEx(&cfg, k_token_logprobs<T, NT>, (const T*)logits, stride, vocab, tokens, top, c, inv_t, split, logprob, entropy, top_logprob, top_token));
-    return VI_OK;
+    return vi::launch_early("k_token_logprobs", k_token_logprobs<T, NT>, dim3((unsigned)(rows * split)), dim3(NT), 0, split, st, (const T*)logits, stride, vocab,
+                            tokens, top, c, inv_t, split, logprob, entropy, top_logprob, top_token);
 }
 
 template <typename T>
