@@ -31,7 +31,7 @@ template <> struct Out<uint64_t> { static __device__ __forceinline__ uint64_t ma
 // ---- tcgen05 ---------------------------------------------------------------------------------------------------
 // A tile is 128 channels by `nt` tokens: the weight is the operand with 128 rows, so a lane of tensor memory is a channel, a
 // column a token, and a warp writes 32 neighbouring channels of one token.
-constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 12;
+constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 12, I8_MAX_SPLIT = 8;
 constexpr int I8_W_BYTES = I8_TN * I8_KS;
 constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, tensor-memory slot, scales of the tokens
 
@@ -48,6 +48,31 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
 // s8 x s8 -> s32; bit 15: the first operand is MN-major
 __device__ __forceinline__ uint32_t idesc_s8(int nt, bool kn) {
     return (2u << 4) | (1u << 7) | (1u << 10) | (kn ? 1u << 15 : 0u) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(I8_TN >> 4) << 24);
+}
+
+// A thread's channel of 16 tokens, `out` the first of them and ldc from each to the next: `tokens` of them exist.
+template <typename T>
+__device__ __forceinline__ void write_out(T* out, int64_t ldc, const uint32_t (&sum)[16], const float* sa, float sb, int tokens) {
+    if (tokens >= 16) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(sa + j);
+            out[0] = Out<T>::make((int)sum[j], a.x, sb);
+            out += ldc;
+            out[0] = Out<T>::make((int)sum[j + 1], a.y, sb);
+            out += ldc;
+            out[0] = Out<T>::make((int)sum[j + 2], a.z, sb);
+            out += ldc;
+            out[0] = Out<T>::make((int)sum[j + 3], a.w, sb);
+            out += ldc;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 15; ++j) {
+            if (j < tokens) out[0] = Out<T>::make((int)sum[j], sa[j], sb);
+            out += ldc;
+        }
+    }
 }
 
 enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
@@ -77,6 +102,8 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
         for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
         mbar_init(accb, 1);
         *abort_flag = 0;
+        prefetch_map(&map_w);
+        prefetch_map(&map_x);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -85,6 +112,9 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     }
     vi::await_inputs();
     for (int j = tid; j < nt; j += I8_THREADS) sa_s[j] = sa && m0 + j < m ? sa[m0 + j] : 1.0f;
+    const int quad = warp & 3, half = warp >> 2;
+    const int64_t ch = n0 + 32 * quad + lane;
+    const float sbv = sb && ch < n ? sb[ch] : 1.0f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -124,33 +154,33 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     if (!ok && *abort_flag == 0) *abort_flag = I8_ERR_ACC;
     tc_fence_after();
     ok = ok && *abort_flag == 0;
-    const int quad = warp & 3, half = warp >> 2;
-    const int64_t ch = n0 + 32 * quad + lane;
-    const float sbv = sb && ch < n ? sb[ch] : 1.0f;
-    auto put = [&](int j, uint32_t v) {
-        if (ch < n && m0 + j < m) C[(m0 + j) * ldc + ch] = Out<T>::make((int)v, sa_s[j], sbv);
-    };
+    T* out = C + m0 * ldc + ch;
+    const int tokens = ch >= n ? 0 : m - m0 < nt ? (int)(m - m0) : nt;
     if (ok) {
         for (int q = half; q < nt / 16; q += 2) {
             uint32_t r[16];
             tmem_ld16(tmem + ((uint32_t)(32 * quad) << 16) + 16 * q, r);
             tmem_ld_wait();
+            if (split == 1) write_out(out + 16 * q * ldc, ldc, r, sa_s + 16 * q, sbv, tokens - 16 * q);
+            else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if (split == 1) put(16 * q + j, r[j]);
-                else ((uint32_t*)base)[(16 * q + j) * I8_TN + 32 * quad + lane] = r[j];
+                for (int j = 0; j < 16; ++j) ((uint32_t*)base)[(16 * q + j) * I8_TN + 32 * quad + lane] = r[j];
             }
         }
     }
     if (split > 1) {
         __syncwarp();
         cluster_sync();
-        const int per = nt / split;
+        const int per = nt / split, j1 = (rank + 1) * per < tokens ? (rank + 1) * per : tokens;
         if (ok) {
-            for (int j = rank * per + half; j < (rank + 1) * per; j += 2) {
-                uint32_t v = 0;
-                for (int p = 0; p < split; ++p) v += cluster_ld(ring + (j * I8_TN + 32 * quad + lane) * 4, p);
-                put(j, v);
+            for (int j = rank * per + half; j < j1; j += 2) {
+                uint32_t part[I8_MAX_SPLIT], v = 0;
+#pragma unroll
+                for (int p = 0; p < I8_MAX_SPLIT; ++p)        // all on their way before the first is added
+                    part[p] = p < split ? cluster_ld(ring + (j * I8_TN + 32 * quad + lane) * 4, p) : 0u;
+#pragma unroll
+                for (int p = 0; p < I8_MAX_SPLIT; ++p) v += part[p];
+                out[j * ldc] = Out<T>::make((int)v, sa_s[j], sbv);
             }
         }
         __syncwarp();
@@ -170,7 +200,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
 // the tokens cross from L2 once a pair.  Two accumulators a block (2 x 256 columns of tensor memory): while eight warps write
 // one tile out, the products of the next one run.
 constexpr int I8_PAIR_THREADS = 320, I8_PAIR_STAGES = 8;
-constexpr int I8_PAIR_TAIL = (2 * I8_PAIR_STAGES + 4 + 1) * 8 + 24;
+constexpr int I8_PAIR_TAIL = (2 * I8_PAIR_STAGES + 4 + 1) * 8 + 24 + 8 * 256 * 4;      // barriers, slots, the tokens' scales for each writing warp
 __host__ __device__ inline int i8_pair_stage_bytes(int nt) { return I8_W_BYTES + nt / 2 * I8_KS; }
 
 template <typename T, bool KN>
@@ -192,6 +222,8 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(acc_full0 + 8 * a, 1); mbar_init(acc_empty0 + 8 * a, 16); }
         *abort_flag = 0;
+        prefetch_map(&map_w);
+        prefetch_map(&map_x);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -257,27 +289,26 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         }
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2;
+        float* sa_s = (float*)(bars + 2 * I8_PAIR_STAGES + 6) + 256 * (warp - 2);      // 16-byte aligned
         int acc = 0;
         uint32_t acc_par = 0;
         for (int t = first; t < tiles; t += step) {
             const int64_t ch = (int64_t)(t / t_tiles) * 2 * I8_TN + rank * I8_TN + 32 * quad + lane, m0 = (int64_t)(t % t_tiles) * nt;
             const float sbv = sb && ch < n ? sb[ch] : 1.0f;
+            __syncwarp();
+            for (int j = lane; j < nt; j += 32) sa_s[j] = sa && m0 + j < m ? sa[m0 + j] : 1.0f;      // while the products run
+            __syncwarp();
             if (!mbar_wait_soon(acc_full0 + 8 * acc, acc_par)) { *abort_flag = I8_ERR_ACC; break; }
             if (*abort_flag) break;
             tc_fence_after();
             const uint32_t from = tmem + 256 * acc + ((uint32_t)(32 * quad) << 16);
             T* out = C + m0 * ldc + ch;
+            const int tokens = ch >= n ? 0 : m - m0 < nt ? (int)(m - m0) : nt;
             for (int q = half; q < nt / 16; q += 2) {
                 uint32_t r[16];
                 tmem_ld16(from + 16 * q, r);
-                const int64_t mine = m0 + 16 * q + (lane & 15);
-                const float sav = sa && mine < m ? sa[mine] : 1.0f;
                 tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float a = __shfl_sync(~0u, sav, j);
-                    if (ch < n && m0 + 16 * q + j < m) out[(16 * q + j) * ldc] = Out<T>::make((int)r[j], a, sbv);
-                }
+                write_out(out + 16 * q * ldc, ldc, r, sa_s + 16 * q, sbv, tokens - 16 * q);
             }
             tc_fence_before();
             __syncwarp();
