@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/verinf_b200.h"
@@ -408,22 +409,46 @@ int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
     return p.by_channel ? launch_pair<T, false>(p, plan, st) : launch_pair<T, true>(p, plan, st);
 }
 
-Plan make_plan(int64_t m, int64_t k, int64_t n) {
-    Plan p;
-    p.pair = m > 256 && n > 256;
-    if (p.pair) {
-        p.nt = 256;
-        p.split = 1;
-        p.stages = 200 * 1024 / i8_pair_stage_bytes(p.nt);
-        return p;
+// Which kernel and tile: the least of estimated times, in us.  The estimate knows what bounds these kernels: the bytes that must
+// come from HBM (6.1 MB a us), the operand bytes of all tiles on their way from L2 to the busiest SM (one at a time 45 KB a us,
+// which is latency, several together 77 KB; in block pairs 59 KB; or the products, 1850 columns a us), a fixed part for set-up
+// and end, the write-out, the second barrier of a split.  Its constants are fitted to 54 shapes (m 1 .. 3986, k 32 .. 11008, n 16
+// .. 11008, both layouts), 746 measured plans: the chosen one takes 0.5 % longer than the best on average, 7 % at worst.
+// Among them: 1 x 4096 x 11008 split 4, 16 tokens 11.4 us, unsplit 13.4; 200 x 4096 x 11008 in pairs 17.3, else 18.4; 200 x
+// 11008 x 4096 split 4, 128 tokens 19.7, in pairs 33; 1000 x 4096 x 11008 in pairs of 224 tokens 38.8, 256 39, single blocks 57.
+Plan make_plan(int m, int k, int n) {
+    const int slices = (k + I8_KS - 1) / I8_KS, n128 = (n + 127) / 128, n256 = (n + 255) / 256;
+    const float hbm = ((float)k * n + (float)m * k + 2.0f * m * n) / 6.14e6f;
+    Plan best = {};
+    float least = 1e30f;
+    static const int widths[] = {16, 32, 48, 64, 96, 128, 192, 256};
+    for (int nt : widths) {
+        if (nt > 16 && nt >= m + 32) break;
+        const int room = nt <= 32 ? 3 : nt <= 128 ? 2 : 1;            // blocks an SM holds
+        const int tiles = (int)std::min<int64_t>((int64_t)((m + nt - 1) / nt) * n128, 1 << 27);
+        for (int split = 1; split <= I8_MAX_SPLIT && (split == 1 || slices >= 2 * split); split *= 2) {
+            const int ctas = tiles * split, steps = (slices + split - 1) / split, rounds = (ctas + 148 * room - 1) / (148 * room);
+            const float bytes = i8_stage_bytes(nt), product = nt / 1850.0f;
+            const float sm = (float)((ctas + 147) / 148) * steps * std::max(bytes / 77e3f, product);
+            const float alone = (float)rounds * steps * std::max(bytes / 45e3f, product);
+            const float t = 2.85f + std::max(hbm, std::max(sm, alone)) + 4.0f * nt / 256 / split * rounds + (split > 1 ? 0.6f : 0.0f) + (rounds - 1);
+            if (t < least) {
+                least = t;
+                const int share = std::min(room, (ctas + 147) / 148);
+                best = {false, nt, split, std::min(I8_MAX_STAGES, (share == 1 ? 200 : nt <= 32 ? 70 : 104) * 1024 / i8_stage_bytes(nt))};
+            }
+        }
     }
-    p.nt = m >= 256 ? 256 : (int)((m + 15) / 16 * 16);
-    const int64_t slices = (k + I8_KS - 1) / I8_KS, tiles = ((m + p.nt - 1) / p.nt) * ((n + I8_TN - 1) / I8_TN);
-    p.split = 1;
-    while (p.split < 8 && tiles * p.split < 148 && slices >= 8 * p.split) p.split *= 2;
-    p.stages = (p.nt <= 32 ? 110 : 200) * 1024 / i8_stage_bytes(p.nt);
-    if (p.stages > I8_MAX_STAGES) p.stages = I8_MAX_STAGES;
-    return p;
+    for (int nt = 32; nt <= 256 && (nt == 32 || nt < m + 32); nt += 32) {
+        const int64_t tiles = (int64_t)((m + nt - 1) / nt) * n256;
+        const float per = (float)((tiles + 73) / 74);
+        const float t = 2.18f + std::max(hbm, per * slices * std::max((16384 + 64 * nt) / 59.4e3f, nt / 925.0f)) + 1.8f * nt / 256;
+        if (t < least) {
+            least = t;
+            best = {true, nt, 1, std::min(I8_PAIR_STAGES, 200 * 1024 / i8_pair_stage_bytes(nt))};
+        }
+    }
+    return best;
 }
 
 // ---- operands that TMA cannot read in place -----------------------------------------------------------------------
@@ -528,7 +553,7 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     Product p = {A, B, lda, ldb, nk, sa, sb, C, ldc, m, k, n};
     const int rc = align_rows(p, (int8_t*)scratch, st);
     if (rc) return rc;
-    const Plan plan = make_plan(m, k, n);
+    const Plan plan = make_plan((int)m, (int)k, (int)n);
     switch (out_type) {
         case VI_F32: return launch_product<float>(p, plan, st);
         case VI_F16: return launch_product<__half>(p, plan, st);
