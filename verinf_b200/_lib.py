@@ -3,7 +3,6 @@
 The library is the only compute path: if it is missing or fails to load, importing
 this module raises — there is no CPU or PyTorch fallback.
 """
-import contextlib
 import ctypes as C
 import os
 from pathlib import Path
@@ -112,17 +111,16 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-_NOTHING = contextlib.nullcontext()
-
-
-def on_device(index: int):
-    """Context in which the device of this index is current: torch.cuda.device, skipped where it is current already."""
-    return _NOTHING if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
-
-
-# torch's current stream of a device index as a number, without the Stream object that torch.cuda.current_stream builds
-# (0.1 us instead of 2.2 us, of some 10 us that a small call takes)
+# torch's current stream of a device index as a number, and an uninitialised tensor (shape, strides, dtype) on the current device,
+# by the calls that torch's own generated code makes: 0.1 us instead of 2.2 us for torch.cuda.current_stream, 0.8 us instead of
+# 2.4 us for torch.empty, of the 10 us that a small call takes.
+current_device = torch._C._cuda_getDevice
 raw_stream = torch._C._cuda_getCurrentRawStream
+try:
+    empty_strided = torch._C._dynamo.guards._empty_strided_cuda
+except AttributeError:
+    def empty_strided(shape, strides, dtype):
+        return torch.empty_strided(shape, strides, dtype=dtype, device="cuda")
 
 
 def ptr(t) -> int:

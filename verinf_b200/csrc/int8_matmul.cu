@@ -32,7 +32,7 @@ template <> struct Out<uint64_t> { static __device__ __forceinline__ uint64_t ma
 // ---- tcgen05 ---------------------------------------------------------------------------------------------------
 // A tile is 128 channels by `nt` tokens: the weight is the operand with 128 rows, so a lane of tensor memory is a channel, a
 // column a token, and a warp writes 32 neighbouring channels of one token.
-constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 12, I8_MAX_SPLIT = 8;
+constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 8, I8_MAX_SPLIT = 8;
 constexpr int I8_W_BYTES = I8_TN * I8_KS;
 constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, tensor-memory slot, scales of the tokens
 
@@ -434,8 +434,7 @@ Plan make_plan(int m, int k, int n) {
             const float t = 2.85f + std::max(hbm, std::max(sm, alone)) + 4.0f * nt / 256 / split * rounds + (split > 1 ? 0.6f : 0.0f) + (rounds - 1);
             if (t < least) {
                 least = t;
-                const int share = std::min(room, (ctas + 147) / 148);
-                best = {false, nt, split, std::min(I8_MAX_STAGES, (share == 1 ? 200 : nt <= 32 ? 70 : 104) * 1024 / i8_stage_bytes(nt))};
+                best = {false, nt, split, (room == 3 ? 70 : room == 2 ? 104 : 200) * 1024 / i8_stage_bytes(nt)};
             }
         }
     }

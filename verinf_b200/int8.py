@@ -12,7 +12,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import LIB, check, on_device, raw_stream
+from ._lib import LIB, check, current_device, empty_strided, raw_stream
 
 # element types of the C ABI (enum in include/verinf_b200.h)
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: 3, torch.uint64: 4}
@@ -60,20 +60,21 @@ def int8_quantize_rows(x, out=None):
     the exact quotient, so that whoever quantises the same row gets the same whole numbers.  A row of zeros has scale 0; one
     that holds a NaN or an infinity has scale NaN and zeros.  `out`: a pair (q, scale) to write into; the rows of q may be any
     distance apart."""
+    index = x.get_device() if isinstance(x, torch.Tensor) else -1
+    if index >= 0 and index != current_device():
+        with torch.cuda.device(index):
+            return int8_quantize_rows(x, out)
     what = "int8_quantize_rows"
     m, k, xs = matrix(x, what, "x", _FLOATS)
-    dev = x.device
     if out is None:
-        q, qs = x.new_empty((m, k), dtype=torch.int8), k
-        scale = x.new_empty(m, dtype=torch.float32)
+        q, qs = empty_strided((m, k), (k, 1), torch.int8), k
+        scale = empty_strided((m,), (1,), torch.float32)
         scale_ptr = scale.data_ptr()
     else:
         q, scale = out
-        qs = _output(q, (m, k), dev, what, "out[0]", _INT8)
-        scale_ptr = _vector(scale, m, dev, what, "out[1]")
-    index = dev.index
-    with on_device(index):
-        rc = LIB.vi_int8_quantize_rows(x.data_ptr(), DTYPE_CODES[x.dtype], m, k, xs, q.data_ptr(), qs, scale_ptr, raw_stream(index))
+        qs = _output(q, (m, k), x.device, what, "out[0]", _INT8)
+        scale_ptr = _vector(scale, m, x.device, what, "out[1]")
+    rc = LIB.vi_int8_quantize_rows(x.data_ptr(), DTYPE_CODES[x.dtype], m, k, xs, q.data_ptr(), qs, scale_ptr, raw_stream(index))
     if rc:
         check(rc)
     return q, scale
@@ -111,13 +112,16 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
     stored by output channel (`weight.t()`), its channels any distance apart.  Rows (channels) that start on 16-byte
     boundaries are read in place; others are copied on every call.  `out`: a tensor of `dtype` to write into, rows any
     distance apart; it must not share memory with the operands."""
+    index = A.get_device() if isinstance(A, torch.Tensor) else -1
+    if index >= 0 and index != current_device():
+        with torch.cuda.device(index):
+            return int8_matmul(A, B, scale_a, scale_b, dtype, out)
     what = "int8_matmul"
     m, k, lda = matrix(A, what, "A", _INT8)
     B, kb, n, by_channel, ldb = _weight(B, what)
-    dev = A.device
     if k != kb:
         raise RuntimeError(f"{what}: inner dim mismatch")
-    if B.device != dev:
+    if B.get_device() != index:
         raise RuntimeError(f"{what}: operands on different devices")
     code = DTYPE_CODES.get(dtype)
     if code is None:
@@ -128,20 +132,19 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
         raise RuntimeError(f"{what}: whole-number outputs take no scales")
     if lda < k:
         A, lda = A.contiguous(), k                      # expanded
-    sa = None if scale_a is None else _vector(scale_a, m, dev, what, "scale_a")
-    sb = None if scale_b is None else _vector(scale_b, n, dev, what, "scale_b")
+    sa = None if scale_a is None else _vector(scale_a, m, A.device, what, "scale_a")
+    sb = None if scale_b is None else _vector(scale_b, n, A.device, what, "scale_b")
     if out is None:
-        out, ldc = A.new_empty((m, n), dtype=dtype), n
+        out, ldc = empty_strided((m, n), (n, 1), dtype), n
     else:
-        ldc = _output(out, (m, n), dev, what, "out", (dtype,))
-    index = dev.index
+        ldc = _output(out, (m, n), A.device, what, "out", (dtype,))
     a, b, room, nb = A.data_ptr(), B.data_ptr(), None, 0
     if (a | b | lda | ldb) & 15:                        # an operand may have to be copied
         nb = LIB.vi_int8_matmul_scratch_bytes(a, lda, b, ldb, by_channel, m, k, n)
-        room = A.new_empty(nb)                          # of the current stream: calls on two streams share nothing
-    with on_device(index):
-        rc = LIB.vi_int8_matmul(a, lda, b, ldb, by_channel, sa, sb, out.data_ptr(), code, ldc, m, k, n,
-                                room.data_ptr() if nb else None, nb, raw_stream(index))
+        if nb:
+            room = empty_strided((nb,), (1,), torch.int8)      # of the current stream: calls on two streams share nothing
+    rc = LIB.vi_int8_matmul(a, lda, b, ldb, by_channel, sa, sb, out.data_ptr(), code, ldc, m, k, n, room.data_ptr() if nb else None,
+                            nb, raw_stream(index))
     if rc:
         check(rc)
     return out

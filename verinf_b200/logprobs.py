@@ -5,7 +5,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import LIB, check, on_device, raw_stream
+from ._lib import LIB, check, current_device, empty_strided, raw_stream
 from .int8 import _FLOATS, DTYPE_CODES, matrix
 
 MAX_TOP = 32
@@ -29,25 +29,26 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     An entry of -inf is a token that is not allowed; a list with fewer allowed tokens than `top` ends in -1 and -inf.  A row of
     -inf alone has logprob -inf, entropy 0 and an empty list.  A row with a NaN or +inf has NaN in its numbers and an empty
     list.  Returns a TokenLogprobs."""
+    index = logits.get_device() if isinstance(logits, torch.Tensor) else -1
+    if index >= 0 and index != current_device():
+        with torch.cuda.device(index):
+            return token_logprobs(logits, tokens, top, temperature)
     what = "token_logprobs"
     rows, vocab, stride = matrix(logits, what, "logits", _FLOATS)
-    dev = logits.device
-    if not isinstance(tokens, torch.Tensor) or tokens.dtype is not torch.int64 or tokens.device != dev or tokens.shape != (rows,) or \
-            not tokens.is_contiguous():
+    if not isinstance(tokens, torch.Tensor) or tokens.dtype is not torch.int64 or tokens.get_device() != index or \
+            tokens.shape != (rows,) or not tokens.is_contiguous():
         raise RuntimeError(f"{what}: tokens must be a contiguous int64 tensor of {rows} tokens on the logits' device")
     if not isinstance(top, int) or not 0 <= top <= MAX_TOP:
         raise RuntimeError(f"{what}: top must be 0 .. {MAX_TOP}")
     if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError(f"{what}: temperature must be between 1e-6 and 1e6")
-    logprob = tokens.new_empty(rows, dtype=torch.float32)
-    entropy = tokens.new_empty(rows, dtype=torch.float32)
-    top_logprob = tokens.new_empty((rows, top), dtype=torch.float32)
-    top_token = tokens.new_empty((rows, top))
-    index = dev.index
-    with on_device(index):
-        rc = LIB.vi_token_logprobs(logits.data_ptr(), DTYPE_CODES[logits.dtype], rows, vocab, stride, tokens.data_ptr(), top,
-                                   temperature, logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr(),
-                                   top_token.data_ptr(), raw_stream(index))
+    logprob = empty_strided((rows,), (1,), torch.float32)
+    entropy = empty_strided((rows,), (1,), torch.float32)
+    top_logprob = empty_strided((rows, top), (top, 1), torch.float32)
+    top_token = empty_strided((rows, top), (top, 1), torch.int64)
+    rc = LIB.vi_token_logprobs(logits.data_ptr(), DTYPE_CODES[logits.dtype], rows, vocab, stride, tokens.data_ptr(), top, temperature,
+                               logprob.data_ptr(), entropy.data_ptr(), top_logprob.data_ptr(), top_token.data_ptr(),
+                               raw_stream(index))
     if rc:
         check(rc)
     return TokenLogprobs(logprob, entropy, top_logprob, top_token)
