@@ -63,7 +63,7 @@ def parse():
     ap.add_argument("--no-secondary", action="store_true",
                     help="skip the 7B-layer commit+sumcheck and the fused K-quant encode on rank 0")
     ap.add_argument("--extra", action="store_true",
-                    help="also run the MoE expert commits, the field matmul and the fold workloads")
+                    help="also run the MoE expert commits, the field matmul, the fold and the quantised head workloads")
     ap.add_argument("--micro", choices=["matmul", "fold", "sumcheck", "int_pipes"],
                     help="run only one secondary kernel (1024 x 2048 x 2048 matmul, the fold of 1024 row pairs "
                          "at K = 16384, or the 2^24 x 3 degree-3 sumcheck) and print its figures; the cases the ncu "
@@ -501,6 +501,7 @@ def run_native(a):
         from verinf_b200 import workloads
         extra["field_matmul"] = workloads.field_matmul(dev)
         extra["fold_products"] = workloads.fold_products(dev)
+        extra["quantised_head"] = workloads.quantised_head(dev)
         if world == 1:          # one GPU only: the reference's extension takes a minute or two to JIT-build
             extra["reference_cuda"] = reference_cuda_leg()
     if a.extra:

@@ -1,6 +1,7 @@
 """Synthetic, seeded end-to-end workloads on top of the kernels (shapes of a Llama-2-7B decoder
 layer; no checkpoint is needed).  Used by `bench.py --extra` to report the secondary figures:
-fused K-quant lift + encode of one MLP weight, and commit + sumcheck of a whole layer.
+fused K-quant lift + encode of one MLP weight, commit + sumcheck of a whole layer, and a review of answered tokens through
+a quantised head.
 
 Layout conventions follow the reference: dense row packing of each flattened tensor into message
 rows of ELL slots (prover/core.py:389-458), production geometry ELL=8192, K=16384, N=65536 with the
@@ -14,9 +15,11 @@ import numpy as np
 import torch
 
 from . import cuda_primitives as cp
+from . import int8
 from . import kquant_cuda as kq
 from . import layergkr_gpu as lg
 from .commit import RowCommitter
+from .logprobs import token_logprobs
 
 P = cp.P
 ELL, K_DEG, N_LIG = 8192, 16384, 65536
@@ -30,8 +33,13 @@ def _signed_to_field(t_int64):
     return out.view(torch.uint64)
 
 
+def _rand_int8(shape, gen, dev):
+    """Random int8 values as int64, the type they are drawn in."""
+    return torch.randint(-128, 128, shape, dtype=torch.int64, device=dev, generator=gen)
+
+
 def _rand_int8_field(shape, gen, dev):
-    return _signed_to_field(torch.randint(-128, 128, shape, dtype=torch.int64, device=dev, generator=gen))
+    return _signed_to_field(_rand_int8(shape, gen, dev))
 
 
 def _pack_rows(flat):
@@ -117,10 +125,15 @@ def field_matmul(dev, m=1000, k=4096, n=11008, seed=5):
     """Witness matmul Y = X W mod p of one MLP projection (gl_matmul, prover/cuda_primitives.py:1086-1106)."""
     g = torch.Generator(device=dev)
     g.manual_seed(seed)
-    X = _rand_int8_field((m, k), g, dev)
-    W = _rand_int8_field((k, n), g, dev)
+    x8, w8 = _rand_int8((m, k), g, dev), _rand_int8((k, n), g, dev)
+    X, W = _signed_to_field(x8), _signed_to_field(w8)
+    x8, w8 = x8.to(torch.int8), w8.to(torch.int8)
     ms = _event_ms(lambda: cp.gl_matmul(X, W))
     out = {"m": m, "k": k, "n": n, "ms": ms, "multiply_adds_per_s": m * k * n / ms * 1e3}
+    # the same field elements from the int8 values themselves
+    out["int8_witness_ms"] = _event_ms(lambda: int8.int8_matmul(x8, w8, dtype=torch.uint64))
+    out["int8_witness_same"] = bool(torch.equal(int8.int8_matmul(x8, w8, dtype=torch.uint64).view(torch.int64),
+                                                cp.gl_matmul(X, W).view(torch.int64)))
     if m > 4 and n > 1:
         out["mma_sync_ms"] = _event_ms(lambda: cp.gl_matmul(X, W, path="mma"))
         out["tcgen05_ms"] = _event_ms(lambda: cp.gl_matmul(X, W, path="umma"))
@@ -168,9 +181,16 @@ def layer7b_commit_sumcheck(dev, seq=1000, seed=11, with_check=False):
     d, dff = 4096, 11008
     shapes = {"W_Q": (d, d), "W_K": (d, d), "W_V": (d, d), "W_O": (d, d), "W_gate": (d, dff), "W_up": (d, dff),
               "W_down": (dff, d)}
-    W = {k: _rand_int8_field(s, g, dev) for k, s in shapes.items()}
-    X = {k: _rand_int8_field((seq, s[0]), g, dev) for k, s in shapes.items()}      # input of each matmul
-    (Y, t_mm) = _timed(lambda: {k: cp.gl_matmul(X[k], W[k]) for k in shapes})
+    W = {k: _rand_int8(s, g, dev) for k, s in shapes.items()}
+    X = {k: _rand_int8((seq, s[0]), g, dev) for k, s in shapes.items()}            # input of each matmul
+    w8, x8 = ({k: t.to(torch.int8) for k, t in d.items()} for d in (W, X))
+    W, X = ({k: _signed_to_field(t) for k, t in d.items()} for d in (W, X))
+    # the witness: field elements from the int8 product (what gl_matmul gives for the lifted operands)
+    witness = lambda: {k: int8.int8_matmul(x8[k], w8[k], dtype=torch.uint64) for k in shapes}
+    witness()                                                     # warm-up, as for the commitments below
+    (Y, t_mm) = _timed(witness)
+    int8.check_async_errors(dev)
+    del w8, x8
     seed_t = torch.arange(32, dtype=torch.uint8, device=dev)
     committers = {}
 
@@ -232,6 +252,34 @@ def layer7b_commit_sumcheck(dev, seq=1000, seed=11, with_check=False):
                    ell=ELL, k=K_DEG, n=N_LIG)
         out["_check"] = chk
     return out
+
+
+def quantised_head(dev, seq=1000, d=4096, vocab=32000, seed=23):
+    """What a review of answered tokens runs: hidden states to int8, the head's int8 product as logits and as the witness that
+    is committed, and how likely the model held each answered token (the bits that it does not explain).  The answers are
+    drawn from the model's own distribution.  Returns stage times, the commitment's root, mean bits and entropy."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    hidden = torch.randn(seq, d, device=dev, generator=g).to(torch.bfloat16)
+    weight, scale_w = int8.int8_quantize_rows(torch.randn(vocab, d, device=dev, generator=g) * (2.5 / d ** 0.5))
+    head = weight.t()                                             # stored by output channel
+    q, scale = int8.int8_quantize_rows(hidden)
+    logits = int8.int8_matmul(q, head, scale, scale_w, dtype=torch.float32)
+    noise = -torch.log(-torch.log(torch.rand(seq, vocab, device=dev, generator=g).clamp_(1e-20, 1 - 1e-7)))
+    tokens = (logits + noise).argmax(1)
+    answers = token_logprobs(logits, tokens, top=20)
+    rows = _pack_rows(int8.int8_matmul(q, head, dtype=torch.uint64).reshape(-1))
+    committer = RowCommitter(rows.size(0), ELL, K_DEG, N_LIG, master_seed=torch.arange(32, dtype=torch.uint8, device=dev), device=dev)
+    root = bytes(committer.commit(rows).cpu().tolist())
+    int8.check_async_errors(dev)
+    return {"seq": seq, "d": d, "vocab": vocab, "rows_committed": rows.size(0),
+            "quantise_ms": _event_ms(lambda: int8.int8_quantize_rows(hidden)),
+            "logits_ms": _event_ms(lambda: int8.int8_matmul(q, head, scale, scale_w, dtype=torch.float32)),
+            "logprobs_ms": _event_ms(lambda: token_logprobs(logits, tokens, top=20)),
+            "witness_ms": _event_ms(lambda: int8.int8_matmul(q, head, dtype=torch.uint64)),
+            "commit_ms": _event_ms(lambda: committer.commit(rows)),
+            "mean_bits": float(-answers.logprob.double().mean() / np.log(2)),
+            "mean_entropy_bits": float(answers.entropy.double().mean() / np.log(2)), "root": root.hex()}
 
 
 def moe_expert_commits(dev, experts, d_ff=5120, d_model=8192, chunk_rows=1024, seed=17, prefix_check=False):
