@@ -111,6 +111,12 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid == 0) {                // the weight's first tiles on their way while the kernel before this one ends
+        for (int s = s0; s < s1 && s < s0 + stages; ++s) {
+            if (KN) prefetch_tile(&map_w, (int32_t)n0, s * I8_KS);
+            else prefetch_tile(&map_w, s * I8_KS, (int32_t)n0);
+        }
+    }
     vi::await_inputs();
     for (int j = tid; j < nt; j += I8_THREADS) sa_s[j] = sa && m0 + j < m ? sa[m0 + j] : 1.0f;
     const int quad = warp & 3, half = warp >> 2;
@@ -230,6 +236,13 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {                // the weight's first tiles on their way while the kernel before this one ends
+        const int32_t n0 = (first / t_tiles) * 2 * I8_TN + rank * I8_TN;
+        for (int s = 0; s < slices && s < stages; ++s) {
+            if (KN) prefetch_tile(&map_w, n0, s * I8_KS);
+            else prefetch_tile(&map_w, s * I8_KS, n0);
+        }
     }
     vi::await_inputs();
     tc_fence_before();
