@@ -55,18 +55,17 @@ __device__ __forceinline__ uint32_t idesc_s8(int nt, bool kn) {
 template <typename T>
 __device__ __forceinline__ void write_out(T* out, int64_t ldc, const uint32_t (&sum)[16], const float* sa, float sb, int tokens) {
     if (tokens >= 16) {
+        T v[16];
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             const float4 a = *reinterpret_cast<const float4*>(sa + j);
-            out[0] = Out<T>::make((int)sum[j], a.x, sb);
-            out += ldc;
-            out[0] = Out<T>::make((int)sum[j + 1], a.y, sb);
-            out += ldc;
-            out[0] = Out<T>::make((int)sum[j + 2], a.z, sb);
-            out += ldc;
-            out[0] = Out<T>::make((int)sum[j + 3], a.w, sb);
-            out += ldc;
+            v[j] = Out<T>::make((int)sum[j], a.x, sb);
+            v[j + 1] = Out<T>::make((int)sum[j + 1], a.y, sb);
+            v[j + 2] = Out<T>::make((int)sum[j + 2], a.z, sb);
+            v[j + 3] = Out<T>::make((int)sum[j + 3], a.w, sb);
         }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[j * ldc] = v[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 15; ++j) {
