@@ -583,3 +583,118 @@ def test_answers_of_a_quantised_head(i8, lp, m):
     as_bits = lambda t: t.view(torch.int64) if t.dtype == torch.uint64 else t
     for a, b, c in zip(first, again, captured):
         assert torch.equal(as_bits(a), as_bits(b)) and torch.equal(as_bits(a), as_bits(c))
+
+
+@gpu
+def test_two_streams_at_once(i8, lp):
+    """Calls on two streams share nothing, operands that have to be copied first among them."""
+    g = torch.Generator().manual_seed(4)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    work = []
+    for j in range(2):
+        A, B = _rand8(g, 120 + j, 1001).cuda(), _weight(g, 1001, 515 + j, ("kn", "nk")[j], 0)
+        x = torch.randn(70, 5003 + j, generator=g).cuda()
+        t = torch.randint(0, 5003, (70,), generator=g).cuda()
+        work.append((A, B, x, t))
+    torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(6):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                A, B, x, t = work[j]
+                results[j].append((i8.int8_matmul(A, B), i8.int8_quantize_rows(x)[0], lp.token_logprobs(x, t, top=7)))
+    torch.cuda.synchronize()
+    for j in range(2):
+        A, B, x, t = work[j]
+        S, q = _sums_64(A, B), _quantize_64(x)[0]
+        for y, qq, out in results[j]:
+            assert torch.equal(y.cpu().long(), S) and torch.equal(qq.cpu(), q)
+            assert all(torch.equal(a, b) for a, b in zip(out, results[j][0][2]))
+        _check_logprobs(lp, x, t, 7)
+
+
+@gpu
+def test_two_graphs_of_one_product(i8):
+    """Two captured products, of operands that have to be copied, replayed in turn and at once, keep their own copies."""
+    g = torch.Generator().manual_seed(6)
+    A = [_rand8(g, 33, 515).cuda() for _ in range(2)]
+    B = [_weight(g, 515, 301, "kn", 0) for _ in range(2)]
+    graphs, outs = [], []
+    for j in range(2):
+        i8.int8_matmul(A[j], B[j])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(i8.int8_matmul(A[j], B[j]))
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        graphs[0].replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for j in range(2):
+            assert torch.equal(outs[j].cpu().long(), _sums_64(A[j], B[j]))
+            A[j].copy_(_rand8(g, 33, 515))
+
+
+@gpu
+def test_offsets_past_32_bits(i8, lp):
+    """Matrices of more than 2^32 entries, looked at in their first and last rows."""
+    x = torch.zeros(70000, 65536, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    ends = [0, 1, 65535, 65536, 69998, 69999]
+    x[ends] = torch.randn(len(ends), 65536, generator=g, device="cuda").bfloat16()
+    q, s = i8.int8_quantize_rows(x)
+    wq, ws = _quantize_64(x[ends])
+    assert torch.equal(q[ends].cpu(), wq) and torch.equal(s[ends].cpu(), ws) and int(q.count_nonzero(1).sum()) == int((wq != 0).sum())
+    tokens = torch.arange(70000, device="cuda") % 65536
+    out = lp.token_logprobs(x, tokens, top=3)
+    part = lp.token_logprobs(x[ends].contiguous(), tokens[ends].contiguous(), top=3)
+    assert all(torch.equal(a[ends], b) for a, b in zip(out, part))
+    assert torch.equal(out.top_token[2], torch.tensor([0, 1, 2], device="cuda"))
+    del x, q, out
+    A = torch.randint(-128, 128, (140000, 64), generator=g, device="cuda", dtype=torch.int8)
+    B = torch.randint(-128, 128, (64, 32768), generator=g, device="cuda", dtype=torch.int8)
+    y = i8.int8_matmul(A, B)
+    ends = [0, 65535, 65536, 131071, 131072, 139999]
+    assert torch.equal(y[ends].cpu().long(), _sums_64(A[ends], B))
+
+
+@gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_other_device_than_the_current_one(i8, lp):
+    g = torch.Generator().manual_seed(4)
+    with torch.cuda.device(0):
+        x = torch.randn(9, 300, generator=g).to("cuda:1")
+        q, s = i8.int8_quantize_rows(x)
+        y = i8.int8_matmul(q, q.t())
+        out = lp.token_logprobs(x, torch.zeros(9, dtype=torch.int64, device="cuda:1"), top=2)
+        assert q.device == y.device == out.entropy.device == x.device and torch.cuda.current_device() == 0
+        assert torch.equal(y.cpu().long(), _sums_64(q, q.t()))
+        with pytest.raises(RuntimeError, match="different devices"):
+            i8.int8_matmul(q, q.t().to("cuda:0"))
+
+
+@gpu
+def test_no_wait_expired(i8):
+    i8.check_async_errors()
+
+
+@gpu
+def test_quantised_head_workload():
+    """The review of answered tokens at a small size: the committed witness is that of the field product."""
+    from verinf_b200 import cuda_primitives as cp, int8, workloads as w
+    dev = torch.device("cuda:0")
+    out = w.quantised_head(dev, seq=40, d=256, vocab=1000, seed=3)
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    hidden = torch.randn(40, 256, device=dev, generator=g).to(torch.bfloat16)
+    weight, _ = int8.int8_quantize_rows(torch.randn(1000, 256, device=dev, generator=g) * (2.5 / 16))
+    q, _ = int8.int8_quantize_rows(hidden)
+    lift = lambda t: w._signed_to_field(t.to(torch.int64)).contiguous()
+    rows = w._pack_rows(cp.gl_matmul(lift(q), lift(weight.t().contiguous())).reshape(-1))
+    root, _, _ = cp.commit_rows(rows, w.K_DEG, w.N_LIG, master_seed=torch.arange(32, dtype=torch.uint8, device=dev))
+    assert bytes(root.cpu().tolist()).hex() == out["root"]
+    assert 0 < out["mean_entropy_bits"] < math.log2(1000) and out["mean_bits"] > 0

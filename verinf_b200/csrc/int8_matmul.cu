@@ -548,6 +548,7 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     VI_REQUIRE(((uintptr_t)sa) % 4 == 0 && ((uintptr_t)sb) % 4 == 0, "int8_matmul: misaligned scales");
     VI_REQUIRE(m < (int64_t(1) << 31) && n < (int64_t(1) << 31), "int8_matmul: m and n are limited to 2^31 - 1");
     cudaStream_t st = (cudaStream_t)stream;
+    if (m == 1) ldc = n;
     if (k == 0) {
         VI_CUDA(cudaMemset2DAsync(C, (size_t)(ldc * out_bytes[out_type]), 0, (size_t)(n * out_bytes[out_type]), (size_t)m, st));
         return VI_OK;

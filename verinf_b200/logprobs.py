@@ -40,6 +40,7 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
         raise RuntimeError(f"{what}: tokens must be a contiguous int64 tensor of {rows} tokens on the logits' device")
     if not isinstance(top, int) or not 0 <= top <= MAX_TOP:
         raise RuntimeError(f"{what}: top must be 0 .. {MAX_TOP}")
+    temperature = float(temperature)
     if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError(f"{what}: temperature must be between 1e-6 and 1e6")
     logprob = empty_strided((rows,), (1,), torch.float32)
