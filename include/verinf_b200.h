@@ -337,8 +337,9 @@ int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_
  * out_type VI_F32 / VI_F16 / VI_BF16: C_ij = (S_ij * sa_i) * sb_j in fp32, rounded once to the type (sa (m), sb (n); NULL =
  * ones); VI_I32: S; VI_FIELD: S mod p as uint64_t, negative sums as p - |S| (the same value vi_gl_matmul gives for the
  * lifted operands); these two take no scales.  C rows ldc elements apart; C must not overlap an operand.
- * An operand whose rows (channels) all start on 16-byte boundaries is read in place, another one is first copied to the
- * scratch: vi_int8_matmul_scratch_bytes (0 when both are read in place), 16-byte aligned.
+ * Operands whose rows (channels) all start on 16-byte boundaries are read in place; others are shifted on their way, or,
+ * where that would take longer, first copied to the scratch: vi_int8_matmul_scratch_bytes (0 where nothing is copied),
+ * 16-byte aligned.  Whole 16-byte cells are read, bytes beside a row that lie in its first and last cell among them.
  * vi_int8_matmul_status: *code = non-zero if a product on the current device gave up on one of its bounded waits since the
  * last call (its output is then incomplete); waits for the device. */
 int64_t vi_int8_matmul_scratch_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel,

@@ -76,9 +76,11 @@ def test_matmul_refusals_without_gpu(lib):
     assert call(out=0, sa=p + 1) != 0 and "scales" in _err(lib)
     assert call(lda=3) != 0 and "operand rows overlap" in _err(lib)
     assert call(nk=1, k=5, lda=5) != 0 and "operand rows overlap" in _err(lib)
-    assert call(A=p + 1) != 0 and "scratch" in _err(lib)
+    assert call(A=p + 1, lda=3001, ldb=2001, m=700, k=3001, n=2001, ldc=2001) != 0 and "scratch" in _err(lib)
     assert L.vi_int8_matmul_scratch_bytes(16, 16, 32, 16, 0, 2, 4, 4) == 0
-    assert L.vi_int8_matmul_scratch_bytes(16, 17, 33, 16, 1, 2, 17, 5) == 2 * 32 + 5 * 32
+    assert L.vi_int8_matmul_scratch_bytes(16, 17, 33, 16, 1, 2, 17, 5) == 0          # shifted on the way
+    assert L.vi_int8_matmul_scratch_bytes(16, 3001, 32, 2001, 0, 700, 3001, 2001) == 700 * 3008 + 3001 * 2016
+    assert L.vi_int8_matmul_scratch_bytes(16, 3008, 33, 3008, 1, 700, 3001, 2001) == 2001 * 3008
     assert L.vi_int8_matmul_status(None) != 0 and "null" in _err(lib)
     assert call(m=0, A=None, Cp=None) == 0
     assert call(n=0, A=None, Cp=None) == 0
@@ -291,7 +293,7 @@ def _check_matmul(i8, A, B, dtypes=None, g=None, out_pad=0):
 @pytest.mark.parametrize("layout", ["kn", "nk"])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 16, 8), (2, 3, 5), (7, 33, 9), (1, 4096, 512), (3, 1000, 130), (16, 128, 128),
                                    (17, 257, 129), (31, 515, 1001), (64, 1024, 256), (65, 48, 300), (128, 384, 640), (129, 1001, 515),
-                                   (255, 64, 31), (300, 2048, 384), (513, 640, 272)])
+                                   (255, 64, 31), (300, 2048, 384), (513, 640, 272), (700, 3001, 2001), (2, 1925, 1098), (20, 77, 1125)])
 def test_matmul_sizes(i8, layout, m, k, n):
     g = torch.Generator().manual_seed(m + 31 * k + 101 * n)
     _check_matmul(i8, _rand8(g, m, k).cuda(), _weight(g, k, n, layout, 0), g=g)

@@ -34,11 +34,11 @@ template <> struct Out<uint64_t> { static __device__ __forceinline__ uint64_t ma
 // column a token, and a warp writes 32 neighbouring channels of one token.
 constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 8, I8_MAX_SPLIT = 8;
 constexpr int I8_W_BYTES = I8_TN * I8_KS;
-constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, tensor-memory slot, scales of the tokens
+constexpr int I8_TAIL_BARS = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4, I8_TAIL = I8_TAIL_BARS;      // barriers, tensor-memory slot, scales of the tokens
 
 __device__ int g_i8_status;                                          // first wait that expired, 0 = none
 
-struct Plan { bool pair; int nt, split, stages; };
+struct Plan { bool pair, direct; int nt, split, stages; };
 __host__ __device__ inline int i8_stage_bytes(int nt) { return I8_W_BYTES + nt * I8_KS; }
 
 // 128-byte rows, 128-byte swizzle, groups of 8 rows 1024 bytes apart: K-major tiles (rows = channels or tokens), and tiles
@@ -75,14 +75,87 @@ __device__ __forceinline__ void write_out(T* out, int64_t ldc, const uint32_t (&
     }
 }
 
+// ---- rows off the 16-byte grid ------------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int by) {      // 16 of 32 bytes, from `by` on
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (by & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
+    if (by & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
+    const int bits = 8 * (by & 3);
+    return {__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits)};
+}
+
+__device__ __forceinline__ uint4 first_bytes(const uint4& v, int n) {       // zero from byte n (1 .. 15) on
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int left = n - 4 * i;
+        o[i] = left >= 4 ? w[i] : left <= 0 ? 0u : w[i] & ((1u << (8 * left)) - 1);
+    }
+    return {o[0], o[1], o[2], o[3]};
+}
+
+struct Operands {
+    const int8_t *A, *B;
+    int64_t lda, ldb;
+};
+
+// Tiles of `rows` x 128 bytes whose rows start anywhere, made as TMA with the 128-byte swizzle would bring them.  TMA reads no
+// such rows, but a cp.async reads any cell of the 16-byte grid: the nine cells that hold a row's 128 bytes go to shared memory
+// as they are, some slices ahead, and are shifted from there into place.  Six warps, each with every sixth row from end to end,
+// so that a warp waits for nothing but its own copies.  Only cells with bytes of the row are read.
+constexpr int I8_LOADERS = I8_THREADS / 32 - 2, I8_CELLS = 9, I8_RAW_STAGES = 3, I8_DIRECT_STAGES = 2;
+struct Tile {
+    const int8_t* src;
+    int64_t pitch, row0, rows_end, len;      // first row, end of the rows, bytes of a row
+    int rows;
+};
+// Row r of a warp's rows is row id + 6 r of the tile.  Three rows a step, a lane with one of their 27 cells.
+__device__ __forceinline__ void fetch_cells(const Tile& t, int64_t c0, uint32_t raw, int id, int lane) {
+    const int cell = lane % I8_CELLS, r0 = id + I8_LOADERS * (lane / I8_CELLS);
+    const int64_t rows = t.rows_end - t.row0;
+    const int end = lane >= 3 * I8_CELLS ? 0 : rows < t.rows ? (int)rows : t.rows;
+    uintptr_t row = (uintptr_t)(t.src + (t.row0 + r0) * t.pitch);
+    const uintptr_t step = 3 * I8_LOADERS * t.pitch;
+    uint32_t to = raw + (r0 * I8_CELLS + cell) * 16;
+#pragma unroll 4
+    for (int r = r0; r < end; r += 3 * I8_LOADERS) {
+        const uintptr_t at = ((row + c0) & ~(uintptr_t)15) + 16 * cell;
+        if (at < row + t.len) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
+        row += step;
+        to += 3 * I8_LOADERS * I8_CELLS * 16;
+    }
+}
+// Four rows a step, eight cells of the tile each.  `last`: zero behind the row's end (one of the two operands has to be).
+template <bool LAST>
+__device__ __forceinline__ void shift_cells(const Tile& t, int64_t c0, const uint8_t* raw, uint8_t* dst, int id, int lane) {
+    const int c = lane & 7, r0 = id + I8_LOADERS * (lane >> 3);
+    uint32_t by = (uint32_t)(uintptr_t)(t.src + c0) + (uint32_t)(t.row0 + r0) * (uint32_t)t.pitch;      // low bits of the row's address
+    const uint32_t step = 4 * I8_LOADERS * (uint32_t)t.pitch;
+    const uint4* from = reinterpret_cast<const uint4*>(raw) + r0 * I8_CELLS + c;
+#pragma unroll 2
+    for (int r = r0; r < t.rows; r += 4 * I8_LOADERS) {
+        uint4 v = shifted(from[0], from[1], by & 15);
+        if (LAST) {
+            const int64_t left = t.len - c0 - 16 * c;
+            if (left <= 0) v = {0, 0, 0, 0};
+            else if (left < 16) v = first_bytes(v, (int)left);
+        }
+        *reinterpret_cast<uint4*>(dst + r * 128 + ((c ^ (r & 7)) << 4)) = v;
+        by += step;
+        from += 4 * I8_LOADERS * I8_CELLS;
+    }
+}
+
 enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
 
 // One tile a block, or, with split > 1, one tile a cluster whose blocks each take a share of the terms; the sums meet through
 // distributed shared memory (whole numbers: the order does not matter).
-template <typename T, bool KN>
-__global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+// DIRECT: operands off the 16-byte grid, brought by warps 2 .. 7 instead of TMA.
+template <typename T, bool KN, bool DIRECT>
+__global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Operands in,
                                                           const float* __restrict__ sa, const float* __restrict__ sb, T* __restrict__ C, int64_t ldc,
-                                                          int64_t m, int64_t n, int t_tiles, int slices, int nt, int split, int stages) {
+                                                          int64_t m, int64_t k, int64_t n, int t_tiles, int slices, int nt, int split, int stages) {
     extern __shared__ uint8_t i8_raw[];
     uint8_t* base = (uint8_t*)(((uintptr_t)i8_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = i8_stage_bytes(nt);
@@ -99,18 +172,20 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     while ((int)cols < nt) cols <<= 1;
 
     if (tid == 0) {
-        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < stages; ++s) { mbar_init(full0 + 8 * s, DIRECT ? I8_LOADERS : 1); mbar_init(empty0 + 8 * s, 1); }
         mbar_init(accb, 1);
         *abort_flag = 0;
-        prefetch_map(&map_w);
-        prefetch_map(&map_x);
+        if (!DIRECT) {
+            prefetch_map(&map_w);
+            prefetch_map(&map_x);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (tid == 0) {                // the weight's first tiles on their way while the kernel before this one ends
+    if (!DIRECT && tid == 0) {     // the weight's first tiles on their way while the kernel before this one ends
         for (int s = s0; s < s1 && s < s0 + stages; ++s) {
             if (KN) prefetch_tile(&map_w, (int32_t)n0, s * I8_KS);
             else prefetch_tile(&map_w, s * I8_KS, (int32_t)n0);
@@ -126,7 +201,39 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
+    if (DIRECT && warp >= 2) {
+        uint8_t* raw = base + stages * stage_bytes + I8_TAIL_BARS;
+        const int raw_bytes = (I8_TN + nt) * I8_CELLS * 16, w_raw = I8_TN * I8_CELLS * 16, id = warp - 2;
+        const Tile x = {in.A, in.lda, m0, m, k, nt};
+        auto weight = [&](int s) { return KN ? Tile{in.B, in.ldb, (int64_t)s * I8_KS, k, n, I8_KS} : Tile{in.B, in.ldb, n0, n, k, I8_TN}; };
+        auto fetch = [&](int s) {
+            if (s < s1) {
+                const uint32_t to = smem_u32(raw) + (s % I8_RAW_STAGES) * raw_bytes;
+                fetch_cells(weight(s), KN ? n0 : (int64_t)s * I8_KS, to, id, lane);
+                fetch_cells(x, (int64_t)s * I8_KS, to + w_raw, id, lane);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int st = 0;
+        uint32_t par = 0;
+        for (int s = s0; s < s0 + I8_RAW_STAGES - 1; ++s) fetch(s);
+        for (int s = s0; s < s1; ++s) {
+            fetch(s + I8_RAW_STAGES - 1);         // into the cells that this warp shifted out of in the step before
+            asm volatile("cp.async.wait_group %0;" ::"n"(I8_RAW_STAGES - 1) : "memory");
+            __syncwarp();
+            if (__any_sync(~0u, s - s0 >= stages && !mbar_wait_soon(empty0 + 8 * st, par ^ 1))) { *abort_flag = I8_ERR_EMPTY; break; }
+            const uint8_t* from = raw + (s % I8_RAW_STAGES) * raw_bytes;
+            uint8_t* dst = base + st * stage_bytes;
+            shift_cells<false>(weight(s), KN ? n0 : (int64_t)s * I8_KS, from, dst, id, lane);
+            if (s + 1 < slices) shift_cells<false>(x, (int64_t)s * I8_KS, from + w_raw, dst + I8_W_BYTES, id, lane);
+            else shift_cells<true>(x, (int64_t)s * I8_KS, from + w_raw, dst + I8_W_BYTES, id, lane);
+            fence_to_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full0 + 8 * st);
+            if (++st == stages) { st = 0; par ^= 1; }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (!DIRECT && warp == 0 && lane == 0) {
         int st = 0;
         uint32_t par = 0;
         for (int s = s0; s < s1; ++s) {
@@ -374,27 +481,23 @@ int grant_smem(const void* kernel, std::atomic<uint64_t>& done) {
     return VI_OK;
 }
 
-template <typename T, bool KN>
+template <typename T, bool KN, bool DIRECT>
 int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
     static std::atomic<uint64_t> granted{0};
-    CUtensorMap map_w, map_x;
-    int rc = KN ? make_map(&map_w, p.B, p.k, p.n, p.ldb, I8_KS) : make_map(&map_w, p.B, p.n, p.k, p.ldb, I8_TN);
-    if (rc) return rc;
-    rc = make_map(&map_x, p.A, p.m, p.k, p.lda, plan.nt);
-    if (rc) return rc;
-    const int smem = plan.stages * i8_stage_bytes(plan.nt) + 1024 + I8_TAIL;
-    rc = grant_smem((const void*)k_int8_umma<T, KN>, granted);
+    CUtensorMap map_w = {}, map_x = {};
+    int rc = VI_OK;
+    if (!DIRECT) {
+        rc = KN ? make_map(&map_w, p.B, p.k, p.n, p.ldb, I8_KS) : make_map(&map_w, p.B, p.n, p.k, p.ldb, I8_TN);
+        if (rc == VI_OK) rc = make_map(&map_x, p.A, p.m, p.k, p.lda, plan.nt);
+    }
+    const int smem = plan.stages * i8_stage_bytes(plan.nt) + 1024 + I8_TAIL + (DIRECT ? I8_RAW_STAGES * (I8_TN + plan.nt) * I8_CELLS * 16 : 0);
+    if (rc == VI_OK) rc = grant_smem((const void*)k_int8_umma<T, KN, DIRECT>, granted);
     if (rc) return rc;
     const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, n_tiles = (p.n + I8_TN - 1) / I8_TN;
     VI_REQUIRE(t_tiles * n_tiles * plan.split <= 0x7FFFFFFF, "int8_matmul: matrix too large for one launch");
-    return vi::launch_early("k_int8_umma", k_int8_umma<T, KN>, dim3((unsigned)(t_tiles * n_tiles * plan.split)), dim3(I8_THREADS), (size_t)smem, plan.split, st,
-                            map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles, (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.split,
-                            plan.stages);
-}
-
-template <typename T>
-int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
-    return p.by_channel ? launch_umma<T, false>(p, plan, st) : launch_umma<T, true>(p, plan, st);
+    return vi::launch_early("k_int8_umma", k_int8_umma<T, KN, DIRECT>, dim3((unsigned)(t_tiles * n_tiles * plan.split)), dim3(I8_THREADS), (size_t)smem,
+                            plan.split, st, map_w, map_x, Operands{p.A, p.B, p.lda, p.ldb}, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.k, p.n, (int)t_tiles,
+                            (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.split, plan.stages);
 }
 
 template <typename T, bool KN>
@@ -417,18 +520,27 @@ int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
 
 template <typename T>
 int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
-    if (!plan.pair) return launch_umma<T>(p, plan, st);
+    if (plan.direct) return p.by_channel ? launch_umma<T, false, true>(p, plan, st) : launch_umma<T, true, true>(p, plan, st);
+    if (!plan.pair) return p.by_channel ? launch_umma<T, false, false>(p, plan, st) : launch_umma<T, true, false>(p, plan, st);
     return p.by_channel ? launch_pair<T, false>(p, plan, st) : launch_pair<T, true>(p, plan, st);
 }
 
 // Which kernel and tile: the least of estimated times, in us.  The estimate knows what bounds these kernels: the bytes that must
-// come from HBM (6.1 MB a us), the operand bytes of all tiles on their way from L2 to the busiest SM (one at a time 45 KB a us,
-// which is latency, several together 77 KB; in block pairs 59 KB; or the products, 1850 columns a us), a fixed part for set-up
-// and end, the write-out, the second barrier of a split.  Its constants are fitted to 54 shapes (m 1 .. 3986, k 32 .. 11008, n 16
-// .. 11008, both layouts), 746 measured plans: the chosen one takes 0.5 % longer than the best on average, 7 % at worst.
-// Among them: 1 x 4096 x 11008 split 4, 16 tokens 11.4 us, unsplit 13.4; 200 x 4096 x 11008 in pairs 17.3, else 18.4; 200 x
-// 11008 x 4096 split 4, 128 tokens 19.7, in pairs 33; 1000 x 4096 x 11008 in pairs of 224 tokens 38.8, 256 39, single blocks 57.
-Plan make_plan(int m, int k, int n) {
+// come from HBM (6.1 MB a us), the operand bytes of all tiles on their way to the busiest SM (one block's at 50 KB a us, which is
+// latency, several blocks' together at 77 KB; a block of a pair at 59 KB) or its products, 1850 columns a us; a fixed part for
+// set-up and end, the write-out, the second barrier of a split, and how many blocks run at once (clusters of 4 and 8 leave SMs
+// unused).  Its constants are fitted to 746 measured plans of 54 shapes (m 1 .. 3986, k 32 .. 11008, n 16 .. 11008, both layouts): the
+// chosen plan takes 0.4 % longer than the best on average, 6 % at worst.  Among them: 1 x 4096 x 11008 split 4, 16 tokens 11.4 us,
+// unsplit 13.4; 200 x 4096 x 11008 in pairs 17.3, else 18.4; 200 x 11008 x 4096 split 4, 128 tokens 19.7, in pairs 33; 1000 x 4096
+// x 11008 in pairs of 224 tokens 38.8, of 256 39, of 128 58, single blocks 57.
+inline int blocks_at_once(int split, int room) { return (split <= 2 ? 148 : split == 4 ? 132 : 120) * room; }
+
+// `off_grid`: bytes of the operands that TMA cannot read in place.  They are copied first (4.7 MB a us, read and written, and a
+// launch more: 4 us, most of it the host's), or, where a tile has few slices, shifted on their way: about 4.4 us for a block's first
+// slice and its end and 1.3 us for each other one, 1.7 us with two blocks an SM (fitted to 406 measured plans of 52 shapes, 9 % off;
+// us with / without a copy, without the host's part: 15 x 77 x 1125 5.8 / 4.7, 2 x 1925 x 1098 8.0 / 6.6, 172 x 581 x 516 7.4 / 8.4,
+// 16 x 11007 x 4095 31 / 25, 100 x 4095 x 11007 36 / 64).
+Plan make_plan(int m, int k, int n, int64_t off_grid) {
     const int slices = (k + I8_KS - 1) / I8_KS, n128 = (n + 127) / 128, n256 = (n + 255) / 256;
     const float hbm = ((float)k * n + (float)m * k + 2.0f * m * n) / 6.14e6f;
     Plan best = {};
@@ -439,24 +551,42 @@ Plan make_plan(int m, int k, int n) {
         const int room = nt <= 32 ? 3 : nt <= 128 ? 2 : 1;            // blocks an SM holds
         const int tiles = (int)std::min<int64_t>((int64_t)((m + nt - 1) / nt) * n128, 1 << 27);
         for (int split = 1; split <= I8_MAX_SPLIT && (split == 1 || slices >= 2 * split); split *= 2) {
-            const int ctas = tiles * split, steps = (slices + split - 1) / split, rounds = (ctas + 148 * room - 1) / (148 * room);
+            const int ctas = tiles * split, steps = (slices + split - 1) / split;
+            const int spread = blocks_at_once(split, 1), rounds = (ctas + spread * room - 1) / (spread * room);
             const float bytes = i8_stage_bytes(nt), product = nt / 1850.0f;
-            const float sm = (float)((ctas + 147) / 148) * steps * std::max(bytes / 77e3f, product);
-            const float alone = (float)rounds * steps * std::max(bytes / 45e3f, product);
+            const float sm = (float)((ctas + spread - 1) / spread) * steps * std::max(bytes / 77e3f, product);
+            const float alone = (float)rounds * steps * std::max(bytes / 50e3f, product);
             const float t = 2.85f + std::max(hbm, std::max(sm, alone)) + 4.0f * nt / 256 / split * rounds + (split > 1 ? 0.6f : 0.0f) + (rounds - 1);
             if (t < least) {
                 least = t;
-                best = {false, nt, split, (room == 3 ? 70 : room == 2 ? 104 : 200) * 1024 / i8_stage_bytes(nt)};
+                best = {false, false, nt, split, (room == 3 ? 70 : room == 2 ? 104 : 200) * 1024 / i8_stage_bytes(nt)};
             }
         }
     }
     for (int nt = 32; nt <= 256 && (nt == 32 || nt < m + 32); nt += 32) {
         const int64_t tiles = (int64_t)((m + nt - 1) / nt) * n256;
         const float per = (float)((tiles + 73) / 74);
-        const float t = 2.18f + std::max(hbm, per * slices * std::max((16384 + 64 * nt) / 59.4e3f, nt / 925.0f)) + 1.8f * nt / 256;
+        const float t = 1.9f + std::max(hbm, per * slices * std::max((16384 + 64 * nt) / 59.4e3f, nt / 925.0f)) + 1.8f * nt / 256;
         if (t < least) {
             least = t;
-            best = {true, nt, 1, std::min(I8_PAIR_STAGES, 200 * 1024 / i8_pair_stage_bytes(nt))};
+            best = {true, false, nt, 1, std::min(I8_PAIR_STAGES, 200 * 1024 / i8_pair_stage_bytes(nt))};
+        }
+    }
+    if (off_grid) {
+        least += 4.0f + 2.0f * off_grid / 4.7e6f;
+        for (int nt : {16, 32, 48, 64, 96, 128}) {
+            if (nt > 16 && nt >= m + 32) break;
+            const int tiles = (int)std::min<int64_t>((int64_t)((m + nt - 1) / nt) * n128, 1 << 27);
+            for (int split = 1; split <= I8_MAX_SPLIT && (split == 1 || slices >= 2 * split); split *= 2) {
+                const int ctas = tiles * split, steps = (slices + split - 1) / split, room = nt <= 32 ? 2 : 1;
+                const int spread = blocks_at_once(split, 1), rounds = (ctas + spread * room - 1) / (spread * room);
+                const float step = (room > 1 && ctas > spread ? 1.7f : 1.3f) * (I8_TN + 0.68f * nt) / 144;
+                const float t = rounds * (0.56f + 3.85f * (I8_TN + nt) / 144 + (steps - 1) * step) + (split > 1 ? 1.5f : 0.0f);
+                if (t < least) {
+                    least = t;
+                    best = {false, true, nt, split, I8_DIRECT_STAGES};
+                }
+            }
         }
     }
     return best;
@@ -473,14 +603,6 @@ struct Rows {
     int8_t* dst;
     int64_t pitch, rows, len;
 };
-
-__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int by) {      // 16 of 32 bytes, from `by` on
-    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    if (by & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
-    if (by & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
-    const int bits = 8 * (by & 3);
-    return {__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits)};
-}
 
 __global__ void __launch_bounds__(256) k_int8_align(const Rows first, const Rows second) {
     vi::await_inputs();
@@ -523,14 +645,18 @@ int align_rows(Product& p, int8_t* room, cudaStream_t st) {
     return vi::launch_early("k_int8_align", k_int8_align, dim3((unsigned)(want < 148 * 32 ? want : 148 * 32), (unsigned)n), dim3(256), 0, 1, st, todo[0], todo[n - 1]);
 }
 
+int64_t copy_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, bool nk, int64_t m, int64_t k, int64_t n) {
+    if (m == 1) lda = 16;                                            // a single row has no next one
+    if (b_rows(k, n, nk) == 1) ldb = 16;
+    return (in_place(A, lda) ? 0 : m * up16(k)) + (in_place(B, ldb) ? 0 : b_rows(k, n, nk) * up16(b_len(k, n, nk)));
+}
+
 }  // namespace
 
 extern "C" int64_t vi_int8_matmul_scratch_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel, int64_t m, int64_t k, int64_t n) {
-    if (m <= 0 || k <= 0 || n <= 0) return 0;
-    if (m == 1) lda = 16;                                            // a single row has no next one
-    if (b_rows(k, n, b_by_channel != 0) == 1) ldb = 16;
-    return (in_place(A, lda) ? 0 : m * up16(k)) +
-           (in_place(B, ldb) ? 0 : b_rows(k, n, b_by_channel != 0) * up16(b_len(k, n, b_by_channel != 0)));
+    if (m <= 0 || k <= 0 || n <= 0 || m > 0x7FFFFFFF || n > 0x7FFFFFFF || k > I8_MAX_K) return 0;
+    const int64_t copies = copy_bytes(A, lda, B, ldb, b_by_channel != 0, m, k, n);
+    return copies && make_plan((int)m, (int)k, (int)n, copies).direct ? 0 : copies;
 }
 
 extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel, const float* sa, const float* sb,
@@ -558,14 +684,17 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     if (b_rows(k, n, nk) == 1) ldb = up16(b_len(k, n, nk));
     VI_REQUIRE(lda >= k && ldb >= b_len(k, n, nk), "int8_matmul: operand rows overlap");
     VI_REQUIRE(lda < (int64_t(1) << 40) && ldb < (int64_t(1) << 40), "int8_matmul: rows too far apart");
-    const int64_t need = vi_int8_matmul_scratch_bytes(A, lda, B, ldb, b_by_channel, m, k, n);
+    const int64_t copies = copy_bytes(A, lda, B, ldb, nk, m, k, n);
+    const Plan plan = make_plan((int)m, (int)k, (int)n, copies);
+    const int64_t need = plan.direct ? 0 : copies;
     if (need && (scratch == nullptr || scratch_bytes < need))
         return vi::fail(VI_ERR_SCRATCH, "int8_matmul: scratch of at least %lld bytes required (see vi_int8_matmul_scratch_bytes)", (long long)need);
     VI_REQUIRE(!need || ((uintptr_t)scratch) % 16 == 0, "int8_matmul: scratch must be 16-byte aligned");
     Product p = {A, B, lda, ldb, nk, sa, sb, C, ldc, m, k, n};
-    const int rc = align_rows(p, (int8_t*)scratch, st);
-    if (rc) return rc;
-    const Plan plan = make_plan((int)m, (int)k, (int)n);
+    if (need) {
+        const int rc = align_rows(p, (int8_t*)scratch, st);
+        if (rc) return rc;
+    }
     switch (out_type) {
         case VI_F32: return launch_product<float>(p, plan, st);
         case VI_F16: return launch_product<__half>(p, plan, st);

@@ -110,7 +110,7 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
 
     The rows of A may be any distance apart.  B is row-major with rows any distance apart, or the transposed view of a weight
     stored by output channel (`weight.t()`), its channels any distance apart.  Rows (channels) that start on 16-byte
-    boundaries are read in place; others are copied on every call.  `out`: a tensor of `dtype` to write into, rows any
+    boundaries are fastest; others are shifted on their way or copied, on every call.  `out`: a tensor of `dtype` to write into, rows any
     distance apart; it must not share memory with the operands."""
     index = A.get_device() if isinstance(A, torch.Tensor) else -1
     if index >= 0 and index != current_device():
