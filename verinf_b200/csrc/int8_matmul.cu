@@ -496,7 +496,7 @@ int launch_umma(const Product& p, const Plan& plan, cudaStream_t st) {
     const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, n_tiles = (p.n + I8_TN - 1) / I8_TN;
     VI_REQUIRE(t_tiles * n_tiles * plan.split <= 0x7FFFFFFF, "int8_matmul: matrix too large for one launch");
     return vi::launch_early("k_int8_umma", k_int8_umma<T, KN, DIRECT>, dim3((unsigned)(t_tiles * n_tiles * plan.split)), dim3(I8_THREADS), (size_t)smem,
-                            plan.split, st, map_w, map_x, Operands{p.A, p.B, p.lda, p.ldb}, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.k, p.n, (int)t_tiles,
+                            plan.split, true, st, map_w, map_x, Operands{p.A, p.B, p.lda, p.ldb}, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.k, p.n, (int)t_tiles,
                             (int)((p.k + I8_KS - 1) / I8_KS), plan.nt, plan.split, plan.stages);
 }
 
@@ -513,7 +513,7 @@ int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
     if (rc) return rc;
     const int64_t t_tiles = (p.m + plan.nt - 1) / plan.nt, tiles = t_tiles * ((p.n + 2 * I8_TN - 1) / (2 * I8_TN));
     VI_REQUIRE(tiles <= 0x3FFFFFFF, "int8_matmul: matrix too large for one launch");
-    return vi::launch_early("k_int8_pair", k_int8_pair<T, KN>, dim3((unsigned)(2 * (tiles < 74 ? tiles : 74))), dim3(I8_PAIR_THREADS), (size_t)smem, 2, st,
+    return vi::launch_early("k_int8_pair", k_int8_pair<T, KN>, dim3((unsigned)(2 * (tiles < 74 ? tiles : 74))), dim3(I8_PAIR_THREADS), (size_t)smem, 2, true, st,
                             map_w, map_x, p.sa, p.sb, (T*)p.C, p.ldc, p.m, p.n, (int)t_tiles, (int)tiles, (int)((p.k + I8_KS - 1) / I8_KS), plan.nt,
                             plan.stages);
 }
@@ -642,7 +642,7 @@ int align_rows(Product& p, int8_t* room, cudaStream_t st) {
     if (n == 0) return VI_OK;
     const int64_t cells0 = todo[0].rows * (up16(todo[0].len) / 16), cells1 = n > 1 ? todo[1].rows * (up16(todo[1].len) / 16) : 0;
     const int64_t want = ((cells0 > cells1 ? cells0 : cells1) + 255) / 256;
-    return vi::launch_early("k_int8_align", k_int8_align, dim3((unsigned)(want < 148 * 32 ? want : 148 * 32), (unsigned)n), dim3(256), 0, 1, st, todo[0], todo[n - 1]);
+    return vi::launch_early("k_int8_align", k_int8_align, dim3((unsigned)(want < 148 * 32 ? want : 148 * 32), (unsigned)n), dim3(256), 0, 1, true, st, todo[0], todo[n - 1]);
 }
 
 int64_t copy_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, bool nk, int64_t m, int64_t k, int64_t n) {

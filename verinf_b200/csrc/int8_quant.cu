@@ -260,7 +260,7 @@ int launch(const void* x, int64_t m, int64_t k, int64_t x_stride, int8_t* q, int
     const unsigned rows = nt == 32 ? 8 : 1;
     const bool aligned = ((uintptr_t)x) % 16 == 0 && x_stride % N == 0 && ((uintptr_t)q) % N == 0 && q_stride % N == 0;
     return vi::launch_early("k_int8_quantize", aligned ? k_int8_quantize<T, true> : k_int8_quantize<T, false>, dim3((unsigned)((m + rows - 1) / rows)),
-                            dim3(nt, rows), 0, 1, st, (const T*)x, x_stride, m, k, q, q_stride, scale);
+                            dim3(nt, rows), 0, 1, true, st, (const T*)x, x_stride, m, k, q, q_stride, scale);
 }
 
 }  // namespace

@@ -15,10 +15,10 @@ __device__ __forceinline__ void await_inputs() { asm volatile("griddepcontrol.wa
 __device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... Params, typename... Args>
-int launch_early(const char* what, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, Args... args) {
+int launch_early(const char* what, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, bool early, cudaStream_t st, Args... args) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
     cudaLaunchConfig_t cfg = {};

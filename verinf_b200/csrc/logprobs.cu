@@ -449,7 +449,9 @@ struct Plan { int threads, split; };      // split <= threads / 32
 template <typename T, int NT>
 int launch(const void* logits, int64_t rows, int64_t vocab, int64_t stride, const int64_t* tokens, int top, float c, float inv_t, float* logprob,
            float* entropy, float* top_logprob, int64_t* top_token, int split, cudaStream_t st) {
-    return vi::launch_early("k_token_logprobs", k_token_logprobs<T, NT>, dim3((unsigned)(rows * split)), dim3(NT), 0, split, st, (const T*)logits, stride, vocab,
+    // Clusters that are placed beside the blocks of the kernel before lie unevenly on the SMs: 64 x 202045 in clusters of four, called
+    // one after the other, 17.6 us when set up early, 14.6 us when not.
+    return vi::launch_early("k_token_logprobs", k_token_logprobs<T, NT>, dim3((unsigned)(rows * split)), dim3(NT), 0, split, split == 1, st, (const T*)logits, stride, vocab,
                             tokens, top, c, inv_t, split, logprob, entropy, top_logprob, top_token);
 }
 
