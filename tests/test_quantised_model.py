@@ -616,6 +616,60 @@ def test_two_streams_at_once(i8, lp):
 
 
 @gpu
+def test_pairs_beside_clusters(i8):
+    """A product of pairs of blocks and one whose terms are shared by clusters, small enough to lie on the same SMs, on two
+    streams at once, many times: neither waits for tensor memory that the other holds while it waits."""
+    g = torch.Generator().manual_seed(12)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    work = [(_rand8(g, 32, 512).cuda(), _weight(g, 512, 18944, "nk", 0)), (_rand8(g, 16, 4096).cuda(), _weight(g, 4096, 1024, "nk", 0))]
+    torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(60):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                results[j].append(i8.int8_matmul(*work[j]))
+    torch.cuda.synchronize()
+    i8.check_async_errors()
+    for (A, B), ys in zip(work, results):
+        S = _sums_64(A, B)
+        assert all(torch.equal(y.cpu().long(), S) for y in ys)
+
+
+@gpu
+def test_captured_streams_that_join(i8, lp):
+    """A captured product whose operands are quantised on two streams that join, one of them from a copied tensor."""
+    g = torch.Generator().manual_seed(13)
+    x, y = torch.zeros(40, 512, device="cuda"), torch.zeros(300, 512, device="cuda")
+    host = torch.zeros(300, 512).pin_memory()
+    tokens = torch.zeros(40, dtype=torch.int64, device="cuda")
+
+    def step():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y.copy_(host, non_blocking=True)
+            wq, ws = i8.int8_quantize_rows(y)
+        q, s = i8.int8_quantize_rows(x)
+        torch.cuda.current_stream().wait_stream(side)
+        logits = i8.int8_matmul(q, wq.t(), s, ws, dtype=torch.float32)
+        return (q, wq, i8.int8_matmul(q, wq.t()), logits) + tuple(lp.token_logprobs(logits, tokens, top=3))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, wq, sums, logits, *_ = out = step()
+    for _ in range(3):
+        x.copy_(torch.randn(40, 512, generator=g))
+        host.copy_(torch.randn(300, 512, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q.cpu(), _quantize_64(x)[0]) and torch.equal(wq.cpu(), _quantize_64(host)[0])
+        assert torch.equal(sums.cpu().long(), _sums_64(q, wq.t()))
+        assert all(torch.equal(a, b) for a, b in zip(out[4:], lp.token_logprobs(logits, tokens, top=3)))
+
+
+@gpu
 def test_two_graphs_of_one_product(i8):
     """Two captured products, of operands that have to be copied, replayed in turn and at once, keep their own copies."""
     g = torch.Generator().manual_seed(6)

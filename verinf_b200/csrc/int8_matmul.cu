@@ -147,6 +147,10 @@ __device__ __forceinline__ void shift_cells(const Tile& t, int64_t c0, const uin
     }
 }
 
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
 enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
 
 // One tile a block, or, with split > 1, one tile a cluster whose blocks each take a share of the terms; the sums meet through
@@ -282,6 +286,11 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
         }
     }
     if (split > 1) {
+        // This block's tensor memory is free before it waits for the others: two blocks of a pair on another stream, each beside
+        // a block of this cluster, could otherwise hold what one of them waits for while the other waits for theirs.
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 1 && *abort_flag == 0) tmem_free(tmem, cols);
         __syncwarp();
         cluster_sync();
         const int per = nt / split, j1 = (rank + 1) * per < tokens ? (rank + 1) * per : tokens;
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    if (warp == 1 && (split == 1 || *abort_flag)) tmem_free(tmem, cols);
 }
 
 // ---- pairs of blocks, persistent --------------------------------------------------------------------------------
