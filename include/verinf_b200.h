@@ -332,7 +332,7 @@ enum { VI_F32 = 0, VI_F16 = 1, VI_BF16 = 2, VI_I32 = 3, VI_FIELD = 4 };
 int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t x_stride,
                           int8_t* q, int64_t q_stride, float* scale, void* stream);
 
-/* S = A.B of int8 matrices, exact in 32 bits (k <= 131071).  A (m, k), rows lda bytes apart; B (k, n) with rows ldb bytes
+/* S = A.B of int8 matrices, exact in 32 bits (k <= 131071; m and n up to 2^31 - 256).  A (m, k), rows lda bytes apart; B (k, n) with rows ldb bytes
  * apart, or, with b_by_channel, stored (n, k) with the k values of a channel together and channels ldb bytes apart.
  * out_type VI_F32 / VI_F16 / VI_BF16: C_ij = (S_ij * sa_i) * sb_j in fp32, rounded once to the type (sa (m), sb (n); NULL =
  * ones); VI_I32: S; VI_FIELD: S mod p as uint64_t, negative sums as p - |S| (the same value vi_gl_matmul gives for the

@@ -86,6 +86,18 @@ def test_matmul_refusals_without_gpu(lib):
     assert call(n=0, A=None, Cp=None) == 0
 
 
+def test_matmul_size_limits_without_gpu(lib):
+    """Sizes whose last tile would end beyond 31-bit indices are refused; the scratch of the largest allowed ones is known."""
+    L = lib.LIB
+    keep, p = _buf()
+    most = (1 << 31) - 256
+    for m, n in [(most + 1, 16), (16, most + 1), (1 << 40, 1)]:
+        assert L.vi_int8_matmul_scratch_bytes(p + 1, 17, p, 16, 1, m, 16, n) == 0
+        assert L.vi_int8_matmul(p + 1, 17, p, 16, 1, None, None, p, 3, n, m, 16, n, None, 0, None) != 0 and "2^31 - 256" in _err(lib)
+    assert L.vi_int8_matmul_scratch_bytes(p + 1, 131072, 16, 131072, 1, most, 131071, 16) == most * 131072
+    assert L.vi_int8_matmul_scratch_bytes(16, 131072, 16, 131072, 1, most, 131071, most) == 0
+
+
 def test_logprobs_refusals_without_gpu(lib):
     L = lib.LIB
     keep, p = _buf()

@@ -18,7 +18,7 @@ namespace {
 
 using namespace vumma;
 
-constexpr int64_t I8_MAX_K = 131071;
+constexpr int64_t I8_MAX_K = 131071, I8_MAX_MN = (int64_t(1) << 31) - 256;      // tiles that reach beyond the end keep 31-bit indices
 constexpr int I8_MAX_SMEM = 227 * 1024;
 
 template <typename T> struct Out;
@@ -663,7 +663,7 @@ int64_t copy_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, b
 }  // namespace
 
 extern "C" int64_t vi_int8_matmul_scratch_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel, int64_t m, int64_t k, int64_t n) {
-    if (m <= 0 || k <= 0 || n <= 0 || m > 0x7FFFFFFF || n > 0x7FFFFFFF || k > I8_MAX_K) return 0;
+    if (m <= 0 || k <= 0 || n <= 0 || m > I8_MAX_MN || n > I8_MAX_MN || k > I8_MAX_K) return 0;
     const int64_t copies = copy_bytes(A, lda, B, ldb, b_by_channel != 0, m, k, n);
     return copies && make_plan((int)m, (int)k, (int)n, copies).direct ? 0 : copies;
 }
@@ -681,7 +681,7 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     VI_REQUIRE(m == 1 || ldc >= n, "int8_matmul: output rows overlap (stride below n)");
     VI_REQUIRE(k == 0 || (A && B), "int8_matmul: null input");
     VI_REQUIRE(((uintptr_t)sa) % 4 == 0 && ((uintptr_t)sb) % 4 == 0, "int8_matmul: misaligned scales");
-    VI_REQUIRE(m < (int64_t(1) << 31) && n < (int64_t(1) << 31), "int8_matmul: m and n are limited to 2^31 - 1");
+    VI_REQUIRE(m <= I8_MAX_MN && n <= I8_MAX_MN, "int8_matmul: m and n are limited to 2^31 - 256");
     cudaStream_t st = (cudaStream_t)stream;
     if (m == 1) ldc = n;
     if (k == 0) {
