@@ -383,6 +383,23 @@ def test_matmul_empty_and_refusals(i8):
 
 
 @gpu
+@pytest.mark.parametrize("m,n", [(1, 1), (3, 700), (2000, 5)])
+def test_matmul_without_terms(i8, m, n):
+    """k = 0: sums of 0, NaN where a scale is not finite; rows of the output any distance apart."""
+    A, B = torch.empty(m, 0, dtype=torch.int8, device="cuda"), torch.empty(0, n, dtype=torch.int8, device="cuda")
+    sa, sb = torch.ones(m, device="cuda"), torch.full((n,), 2.0, device="cuda")
+    sa[m // 2], sb[n // 2] = math.nan, -math.inf
+    bad = (torch.arange(m) == m // 2)[:, None] | (torch.arange(n) == n // 2)
+    for dtype in FLOATS:
+        room = torch.full((m, n + 3), 7.0, device="cuda", dtype=dtype)
+        y = i8.int8_matmul(A, B, sa, sb, dtype=dtype, out=room[:, :n]).cpu()
+        assert torch.isnan(y[bad]).all() and (y[~bad] == 0).all() and (room[:, n:] == 7).all()
+        assert (i8.int8_matmul(A, B.t().contiguous().t(), dtype=dtype) == 0).all()
+    for dtype in (torch.int32, torch.uint64):
+        assert (i8.int8_matmul(A, B, dtype=dtype).view(torch.int32) == 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("layout", ["kn", "nk"])
 def test_matmul_witness_is_the_field_product(i8, layout):
     from verinf_b200 import cuda_primitives as cp

@@ -34,7 +34,7 @@ template <> struct Out<uint64_t> { static __device__ __forceinline__ uint64_t ma
 // column a token, and a warp writes 32 neighbouring channels of one token.
 constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 8, I8_MAX_SPLIT = 8;
 constexpr int I8_W_BYTES = I8_TN * I8_KS;
-constexpr int I8_TAIL_BARS = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4, I8_TAIL = I8_TAIL_BARS;      // barriers, tensor-memory slot, scales of the tokens
+constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, tensor-memory slot, scales of the tokens
 
 __device__ int g_i8_status;                                          // first wait that expired, 0 = none
 
@@ -154,7 +154,8 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
 enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
 
 // One tile a block, or, with split > 1, one tile a cluster whose blocks each take a share of the terms; the sums meet through
-// distributed shared memory (whole numbers: the order does not matter).
+// distributed shared memory (whole numbers: the order does not matter).  For few tokens, where the weight's bytes and the latency
+// of the first loads and of the join bind: 1 x 4096 x 11008 10.8 us (4.2 TB/s), 16 x 11008 x 4096 11.8 us (3.9 TB/s).
 // DIRECT: operands off the 16-byte grid, brought by warps 2 .. 7 instead of TMA.
 template <typename T, bool KN, bool DIRECT>
 __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Operands in,
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
     const uint32_t tmem = *tmem_slot;
 
     if (DIRECT && warp >= 2) {
-        uint8_t* raw = base + stages * stage_bytes + I8_TAIL_BARS;
+        uint8_t* raw = base + stages * stage_bytes + I8_TAIL;
         const int raw_bytes = (I8_TN + nt) * I8_CELLS * 16, w_raw = I8_TN * I8_CELLS * 16, id = warp - 2;
         const Tile x = {in.A, in.lda, m0, m, k, nt};
         auto weight = [&](int s) { return KN ? Tile{in.B, in.ldb, (int64_t)s * I8_KS, k, n, I8_KS} : Tile{in.B, in.ldb, n0, n, k, I8_TN}; };
@@ -320,7 +321,9 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
 // ---- pairs of blocks, persistent --------------------------------------------------------------------------------
 // A tile is 256 channels by `nt` tokens, 128 channels a block; each block brings its channels and half of the tokens, so that
 // the tokens cross from L2 once a pair.  Two accumulators a block (2 x 256 columns of tensor memory): while eight warps write
-// one tile out, the products of the next one run.
+// one tile out, the products of the next one run.  Bound by the tensor pipe, about 69 % of which is busy while a tile runs, and by
+// the last round of tiles: 1000 x 4096 x 11008 39 us (2.3 P operations a second; 172 tiles on 74 pairs), 4096 x 5120 x 8192 113 us
+// (3.0 P; 512 tiles).
 constexpr int I8_PAIR_THREADS = 320, I8_PAIR_STAGES = 8;
 constexpr int I8_PAIR_TAIL = (2 * I8_PAIR_STAGES + 4 + 1) * 8 + 24 + 8 * 256 * 4;      // barriers, slots, the tokens' scales for each writing warp
 __host__ __device__ inline int i8_pair_stage_bytes(int nt) { return I8_W_BYTES + nt / 2 * I8_KS; }
@@ -456,6 +459,14 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// No terms (k = 0): sums of 0, which a scale that is not finite turns into NaN as it does elsewhere.
+template <typename T>
+__global__ void __launch_bounds__(256) k_int8_no_terms(const float* __restrict__ sa, const float* __restrict__ sb, T* __restrict__ C, int64_t ldc, int64_t m, int64_t n) {
+    vi::await_inputs();
+    for (int64_t i = blockIdx.x; i < m; i += gridDim.x)
+        for (int64_t j = threadIdx.x; j < n; j += 256) C[i * ldc + j] = Out<T>::make(0, sa ? sa[i] : 1.0f, sb ? sb[j] : 1.0f);
+}
+
 // rows x len bytes, rows `pitch` bytes apart; box: 128 bytes x box_rows
 int make_map(CUtensorMap* map, const int8_t* ptr, int64_t rows, int64_t len, int64_t pitch, int box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();
@@ -529,10 +540,16 @@ int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
 
 template <typename T>
 int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
+    if (p.k == 0)
+        return vi::launch_early("k_int8_no_terms", k_int8_no_terms<T>, dim3((unsigned)std::min<int64_t>(p.m, 148 * 8)), dim3(256), 0, 1, true, st, p.sa, p.sb,
+                                (T*)p.C, p.ldc, p.m, p.n);
     if (plan.direct) return p.by_channel ? launch_umma<T, false, true>(p, plan, st) : launch_umma<T, true, true>(p, plan, st);
     if (!plan.pair) return p.by_channel ? launch_umma<T, false, false>(p, plan, st) : launch_umma<T, true, false>(p, plan, st);
     return p.by_channel ? launch_pair<T, false>(p, plan, st) : launch_pair<T, true>(p, plan, st);
 }
+
+// blocks of clusters of `split` that run at once, `room` on an SM
+inline int blocks_at_once(int split, int room) { return (split <= 2 ? 148 : split == 4 ? 132 : 120) * room; }
 
 // Which kernel and tile: the least of estimated times, in us.  The estimate knows what bounds these kernels: the bytes that must
 // come from HBM (6.1 MB a us), the operand bytes of all tiles on their way to the busiest SM (one block's at 50 KB a us, which is
@@ -542,8 +559,7 @@ int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
 // chosen plan takes 0.4 % longer than the best on average, 6 % at worst.  Among them: 1 x 4096 x 11008 split 4, 16 tokens 11.4 us,
 // unsplit 13.4; 200 x 4096 x 11008 in pairs 17.3, else 18.4; 200 x 11008 x 4096 split 4, 128 tokens 19.7, in pairs 33; 1000 x 4096
 // x 11008 in pairs of 224 tokens 38.8, of 256 39, of 128 58, single blocks 57.
-inline int blocks_at_once(int split, int room) { return (split <= 2 ? 148 : split == 4 ? 132 : 120) * room; }
-
+//
 // `off_grid`: bytes of the operands that TMA cannot read in place.  They are copied first (4.7 MB a us, read and written, and a
 // launch more: 4 us, most of it the host's), or, where a tile has few slices, shifted on their way: about 4.4 us for a block's first
 // slice and its end and 1.3 us for each other one, 1.7 us with two blocks an SM (fitted to 406 measured plans of 52 shapes, 9 % off;
@@ -602,8 +618,8 @@ Plan make_plan(int m, int k, int n, int64_t off_grid) {
 }
 
 // ---- operands that TMA cannot read in place -----------------------------------------------------------------------
-// Rows that start off the 16-byte grid are copied to rows that start on it: a pass over those bytes, on every call (11008 rows
-// of 4096 bytes: see below).  A thread makes 16 bytes of the copy from the two grid cells that hold them, of which it reads only
+// Rows that start off the 16-byte grid are copied to rows that start on it: a pass over those bytes, on every call (what it
+// takes: at make_plan).  A thread makes 16 bytes of the copy from the two grid cells that hold them, of which it reads only
 // those that hold bytes of the row.
 inline __host__ __device__ int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
 
@@ -684,17 +700,13 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     VI_REQUIRE(m <= I8_MAX_MN && n <= I8_MAX_MN, "int8_matmul: m and n are limited to 2^31 - 256");
     cudaStream_t st = (cudaStream_t)stream;
     if (m == 1) ldc = n;
-    if (k == 0) {
-        VI_CUDA(cudaMemset2DAsync(C, (size_t)(ldc * out_bytes[out_type]), 0, (size_t)(n * out_bytes[out_type]), (size_t)m, st));
-        return VI_OK;
-    }
     const bool nk = b_by_channel != 0;
     if (m == 1) lda = up16(k);
     if (b_rows(k, n, nk) == 1) ldb = up16(b_len(k, n, nk));
-    VI_REQUIRE(lda >= k && ldb >= b_len(k, n, nk), "int8_matmul: operand rows overlap");
+    VI_REQUIRE(k == 0 || (lda >= k && ldb >= b_len(k, n, nk)), "int8_matmul: operand rows overlap");
     VI_REQUIRE(lda < (int64_t(1) << 40) && ldb < (int64_t(1) << 40), "int8_matmul: rows too far apart");
-    const int64_t copies = copy_bytes(A, lda, B, ldb, nk, m, k, n);
-    const Plan plan = make_plan((int)m, (int)k, (int)n, copies);
+    const int64_t copies = k ? copy_bytes(A, lda, B, ldb, nk, m, k, n) : 0;
+    const Plan plan = k ? make_plan((int)m, (int)k, (int)n, copies) : Plan{};
     const int64_t need = plan.direct ? 0 : copies;
     if (need && (scratch == nullptr || scratch_bytes < need))
         return vi::fail(VI_ERR_SCRATCH, "int8_matmul: scratch of at least %lld bytes required (see vi_int8_matmul_scratch_bytes)", (long long)need);

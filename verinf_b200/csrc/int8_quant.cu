@@ -5,8 +5,8 @@
 // program that quantises the same activations commits to the same whole numbers.
 //
 // Bound by HBM: a row is read once and stays in the registers of its block (up to 128 KB of row), the maximum meets in shared
-// memory, and the row leaves as bytes; a longer row is read twice, the second time from L2.  11008 x 4096 fp32 34 us (6.6 TB/s),
-// bf16 22 us (6.1 TB/s); 1000 x 11008 bf16 8.7 us (3.8 TB/s: one wave of blocks, whose load and store phases hardly overlap).
+// memory, and the row leaves as bytes; a longer row is read twice, the second time from L2.  11008 x 4096 fp32 34 us (6.7 TB/s),
+// bf16 22 us (6.1 TB/s); 1000 x 11008 bf16 7.0 us (4.7 TB/s: one wave of blocks, whose load and store phases hardly overlap).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

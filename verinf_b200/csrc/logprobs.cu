@@ -4,7 +4,8 @@
 // With c = log2(e) / T and a_j = (x_j - max) c:  S = sum 2^a_j, logprob = ln 2 (a_t - log2 S), entropy = ln 2 (log2 S -
 // (sum 2^a_j a_j) / S), alternatives in the order of x (ties to the lowest index).  One pass: a thread keeps the maximum m of
 // its entries, s = sum 2^a and w = sum 2^a a against that maximum, and rescales s and w when the maximum grows; two such
-// triples join in the same way.  The sums are in fp32; a thread adds vocab / 256 terms or fewer.
+// triples join in the same way.  The sums are in fp32; a thread adds vocab / 128 terms or fewer
+// (vocab / 64 of a row of 1024 packs or less), two by two.
 //
 // Alternatives without a second pass: a thread's packs (the entries of one 16-byte load) fall into four shares, and it keeps
 // the largest entry of each share and the pack that first reached it.  The threads form 64 groups, each with the best (value,

@@ -6,7 +6,7 @@ elements: the witness that `gl_matmul` gives for the operands lifted by the sign
 one pass over one byte plane instead of 64 plane products.
 
 As elsewhere in the package: CUDA tensors, outputs allocated with torch (or given as `out`), kernels on torch's current stream
-of the tensors' device, RuntimeError for what is refused.
+of the tensors' device, RuntimeError for what is refused.  Outputs carry no gradient: nothing in the package is trained.
 """
 import ctypes as C
 
@@ -92,6 +92,8 @@ def _weight(B, what):
         raise RuntimeError(f"{what}: B must be 2-D")
     k, n = shape
     s0, s1 = B.stride()
+    if n == 1 and s0 == 1:                              # a column is one channel: a row of k instead of k rows of one
+        return B, k, n, 1, k
     if (s1 == 1 or n == 1) and (s0 >= n or k == 1):
         return B, k, n, 0, s0 if k > 1 else n
     if (s0 == 1 or k == 1) and (s1 >= k or n == 1):
@@ -110,8 +112,8 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
 
     The rows of A may be any distance apart.  B is row-major with rows any distance apart, or the transposed view of a weight
     stored by output channel (`weight.t()`), its channels any distance apart.  Rows (channels) that start on 16-byte
-    boundaries are fastest; others are shifted on their way or copied, on every call.  `out`: a tensor of `dtype` to write into, rows any
-    distance apart; it must not share memory with the operands."""
+    boundaries are fastest; others are shifted on their way or copied, on every call.  `out`: a tensor of `dtype` to write
+    into, rows any distance apart; it must not share memory with the operands."""
     index = A.get_device() if isinstance(A, torch.Tensor) else -1
     if index >= 0 and index != current_device():
         with torch.cuda.device(index):
