@@ -370,21 +370,25 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
+        {
             int st = 0, filled = 0;
-            uint32_t par = 0;
+            uint32_t par = 0, dst = ring;
+            const uint32_t full_first = cluster_addr(full0, 0);       // the pair's first block's
             for (int t = first; t < tiles && !*abort_flag; t += step) {
                 const int32_t n0 = (t / t_tiles) * 2 * I8_TN + rank * I8_TN, m0 = (t % t_tiles) * nt + rank * (nt / 2);
                 for (int s = 0; s < slices; ++s) {
                     if (filled == stages) {
-                        if (!mbar_wait_soon(empty0 + 8 * st, par ^ 1)) { *abort_flag = I8_ERR_EMPTY; break; }
+                        if (__any_sync(~0u, !mbar_wait_soon(empty0 + 8 * st, par ^ 1))) { *abort_flag = I8_ERR_EMPTY; break; }
                     } else ++filled;
-                    const uint32_t dst = ring + st * stage_bytes, fb = cluster_addr(full0 + 8 * st, 0);
-                    if (rank == 0) mbar_expect_tx(full0 + 8 * st, 2 * stage_bytes);
-                    if (KN) tma_load_2d_pair(dst, &map_w, n0, s * I8_KS, fb);
-                    else tma_load_2d_pair(dst, &map_w, s * I8_KS, n0, fb);
-                    tma_load_2d_pair(dst + I8_W_BYTES, &map_x, s * I8_KS, m0, fb);
-                    if (++st == stages) { st = 0; par ^= 1; }
+                    if (elect_one()) {
+                        const uint32_t fb = full_first + 8 * st;
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * st, 2 * stage_bytes);
+                        if (KN) tma_load_2d_pair(dst, &map_w, n0, s * I8_KS, fb);
+                        else tma_load_2d_pair(dst, &map_w, s * I8_KS, n0, fb);
+                        tma_load_2d_pair(dst + I8_W_BYTES, &map_x, s * I8_KS, m0, fb);
+                    }
+                    dst += stage_bytes;
+                    if (++st == stages) { st = 0; par ^= 1; dst = ring; }
                 }
             }
             // the last commits arrive here: stay until they have
@@ -396,26 +400,30 @@ k_int8_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             int st = 0, acc = 0, used = 0;
             uint32_t par = 0, acc_par = 0;
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (KN ? 1u << 15 : 0u) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(2 * I8_TN >> 4) << 24);
+            const uint64_t w0 = desc_sw128(ring), x0 = desc_sw128(ring + I8_W_BYTES);
+            uint32_t at = 0;                                           // of the stage, in the descriptors' 16 bytes
             for (int t = first; t < tiles && !*abort_flag; t += step) {
-                if (used >= 2 && !mbar_wait_soon(acc_empty0 + 8 * acc, acc_par ^ 1)) { *abort_flag = I8_ERR_ACC; break; }
+                if (used >= 2 && __any_sync(~0u, !mbar_wait_soon(acc_empty0 + 8 * acc, acc_par ^ 1))) { *abort_flag = I8_ERR_ACC; break; }
                 ++used;
                 tc_fence_after();
                 const uint32_t d = tmem + 256 * acc;
                 for (int s = 0; s < slices; ++s) {
-                    if (!mbar_wait_soon(full0 + 8 * st, par)) { *abort_flag = I8_ERR_FULL; break; }
+                    if (__any_sync(~0u, !mbar_wait_soon(full0 + 8 * st, par))) { *abort_flag = I8_ERR_FULL; break; }
                     tc_fence_after();
-                    const uint32_t w = ring + st * stage_bytes, x = w + I8_W_BYTES;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < I8_KS / 32; ++kk)
-                        umma_i8_pair(d, desc_sw128(w + kk * (KN ? 32 * 128 : 32)), desc_sw128(x + kk * 32), idesc, s > 0 || kk > 0);
-                    umma_commit_pair(empty0 + 8 * st);
-                    if (++st == stages) { st = 0; par ^= 1; }
+                        for (int kk = 0; kk < I8_KS / 32; ++kk)
+                            umma_i8_pair(d, w0 + at + kk * (KN ? 32 * 128 / 16 : 2), x0 + at + kk * 2, idesc, s > 0 || kk > 0);
+                        umma_commit_pair(empty0 + 8 * st);
+                    }
+                    at += stage_bytes / 16;
+                    if (++st == stages) { st = 0; par ^= 1; at = 0; }
                 }
-                umma_commit_pair(acc_full0 + 8 * acc);
+                if (elect_one()) umma_commit_pair(acc_full0 + 8 * acc);
                 if (++acc == 2) { acc = 0; acc_par ^= 1; }
             }
         }

@@ -57,6 +57,16 @@ __device__ __forceinline__ bool mbar_wait_soon(uint32_t bar, uint32_t parity) {
         }
     }
 }
+// one lane of a converged warp; where it branches on this, the compiler knows that one lane is left and keeps what the lane
+// gives to the tensor cores and TMA in uniform registers
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "elect.sync _|p, 0xFFFFFFFF;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
