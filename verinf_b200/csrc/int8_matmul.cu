@@ -238,32 +238,38 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
             if (++st == stages) { st = 0; par ^= 1; }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (!DIRECT && warp == 0 && lane == 0) {
+    } else if (!DIRECT && warp == 0) {
         int st = 0;
-        uint32_t par = 0;
+        uint32_t par = 0, dst = ring;
         for (int s = s0; s < s1; ++s) {
-            if (s - s0 >= stages && !mbar_wait_soon(empty0 + 8 * st, par ^ 1)) { *abort_flag = I8_ERR_EMPTY; break; }
-            const uint32_t fb = full0 + 8 * st, dst = ring + st * stage_bytes;
-            mbar_expect_tx(fb, stage_bytes);
-            if (KN) tma_load_2d(dst, &map_w, (int32_t)n0, s * I8_KS, fb);
-            else tma_load_2d(dst, &map_w, s * I8_KS, (int32_t)n0, fb);
-            tma_load_2d(dst + I8_W_BYTES, &map_x, s * I8_KS, (int32_t)m0, fb);
-            if (++st == stages) { st = 0; par ^= 1; }
+            if (s - s0 >= stages && __any_sync(~0u, !mbar_wait_soon(empty0 + 8 * st, par ^ 1))) { *abort_flag = I8_ERR_EMPTY; break; }
+            if (elect_one()) {
+                const uint32_t fb = full0 + 8 * st;
+                mbar_expect_tx(fb, stage_bytes);
+                if (KN) tma_load_2d(dst, &map_w, (int32_t)n0, s * I8_KS, fb);
+                else tma_load_2d(dst, &map_w, s * I8_KS, (int32_t)n0, fb);
+                tma_load_2d(dst + I8_W_BYTES, &map_x, s * I8_KS, (int32_t)m0, fb);
+            }
+            dst += stage_bytes;
+            if (++st == stages) { st = 0; par ^= 1; dst = ring; }
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         int st = 0;
-        uint32_t par = 0;
+        uint32_t par = 0, at = 0;                                      // at: the stage, in the descriptors' 16 bytes
         const uint32_t idesc = idesc_s8(nt, KN);
-        for (int s = s0; s < s1 && !*abort_flag; ++s) {
-            if (!mbar_wait_soon(full0 + 8 * st, par)) { *abort_flag = I8_ERR_FULL; break; }
+        const uint64_t w0 = desc_sw128(ring), x0 = desc_sw128(ring + I8_W_BYTES);
+        for (int s = s0; s < s1; ++s) {
+            if (__any_sync(~0u, !mbar_wait_soon(full0 + 8 * st, par))) { *abort_flag = I8_ERR_FULL; break; }
             tc_fence_after();
-            const uint32_t w = ring + st * stage_bytes, x = w + I8_W_BYTES;
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < I8_KS / 32; ++kk)
-                umma_i8(tmem, desc_sw128(w + kk * (KN ? 32 * 128 : 32)), desc_sw128(x + kk * 32), idesc, s > s0 || kk > 0);
-            if (s + stages < s1) umma_commit(empty0 + 8 * st);        // the last ones are not loaded again
-            if (s + 1 == s1) umma_commit(accb);
-            if (++st == stages) { st = 0; par ^= 1; }
+                for (int kk = 0; kk < I8_KS / 32; ++kk)
+                    umma_i8(tmem, w0 + at + kk * (KN ? 32 * 128 / 16 : 2), x0 + at + kk * 2, idesc, s > s0 || kk > 0);
+                if (s + stages < s1) umma_commit(empty0 + 8 * st);        // the last ones are not loaded again
+                if (s + 1 == s1) umma_commit(accb);
+            }
+            at += stage_bytes / 16;
+            if (++st == stages) { st = 0; par ^= 1; at = 0; }
         }
     }
     __syncwarp();
