@@ -650,7 +650,7 @@ def test_pairs_beside_clusters(i8):
     streams at once, many times: neither waits for tensor memory that the other holds while it waits."""
     g = torch.Generator().manual_seed(12)
     streams = [torch.cuda.Stream() for _ in range(2)]
-    work = [(_rand8(g, 32, 512).cuda(), _weight(g, 512, 18944, "nk", 0)), (_rand8(g, 16, 4096).cuda(), _weight(g, 4096, 1024, "nk", 0))]
+    work = [(_rand8(g, 32, 1024).cuda(), _weight(g, 1024, 11008, "nk", 0)), (_rand8(g, 16, 4096).cuda(), _weight(g, 4096, 1024, "nk", 0))]
     torch.cuda.synchronize()
     results = [[], []]
     for _ in range(60):

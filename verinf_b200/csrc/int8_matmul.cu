@@ -155,7 +155,7 @@ enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
 
 // One tile a block, or, with split > 1, one tile a cluster whose blocks each take a share of the terms; the sums meet through
 // distributed shared memory (whole numbers: the order does not matter).  For few tokens, where the weight's bytes and the latency
-// of the first loads and of the join bind: 1 x 4096 x 11008 10.8 us (4.2 TB/s), 16 x 11008 x 4096 11.8 us (3.9 TB/s).
+// of the first loads and of the join bind: 1 x 4096 x 11008 10.6 us (4.3 TB/s), 16 x 11008 x 4096 11.8 us (3.9 TB/s).
 // DIRECT: operands off the 16-byte grid, brought by warps 2 .. 7 instead of TMA.
 template <typename T, bool KN, bool DIRECT>
 __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Operands in,
@@ -327,9 +327,10 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant_
 // ---- pairs of blocks, persistent --------------------------------------------------------------------------------
 // A tile is 256 channels by `nt` tokens, 128 channels a block; each block brings its channels and half of the tokens, so that
 // the tokens cross from L2 once a pair.  Two accumulators a block (2 x 256 columns of tensor memory): while eight warps write
-// one tile out, the products of the next one run.  Bound by the tensor pipe, about 69 % of which is busy while a tile runs, and by
-// the last round of tiles: 1000 x 4096 x 11008 39 us (2.3 P operations a second; 172 tiles on 74 pairs), 4096 x 5120 x 8192 113 us
-// (3.0 P; 512 tiles).
+// one tile out, the products of the next one run.  Bound by the tensor pipe and its feeding, about 0.32 us a slice of 256 tokens (0.26
+// of them the products'): 1000 x 4096 x 11008 35 us (2.6 P operations a second; 215 tiles of 224 tokens on 74 pairs), 4096 x 5120 x
+// 8192 104 us (3.3 P; 512 tiles).  The warps that load and that issue the products run their loops whole and elect the lane that
+// issues: with a loop of one lane each slice costs 0.07 us more (39 and 113 us).
 constexpr int I8_PAIR_THREADS = 320, I8_PAIR_STAGES = 8;
 constexpr int I8_PAIR_TAIL = (2 * I8_PAIR_STAGES + 4 + 1) * 8 + 24 + 8 * 256 * 4;      // barriers, slots, the tokens' scales for each writing warp
 __host__ __device__ inline int i8_pair_stage_bytes(int nt) { return I8_W_BYTES + nt / 2 * I8_KS; }
@@ -566,13 +567,16 @@ int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
 inline int blocks_at_once(int split, int room) { return (split <= 2 ? 148 : split == 4 ? 132 : 120) * room; }
 
 // Which kernel and tile: the least of estimated times, in us.  The estimate knows what bounds these kernels: the bytes that must
-// come from HBM (6.1 MB a us), the operand bytes of all tiles on their way to the busiest SM (one block's at 50 KB a us, which is
-// latency, several blocks' together at 77 KB; a block of a pair at 59 KB) or its products, 1850 columns a us; a fixed part for
-// set-up and end, the write-out, the second barrier of a split, and how many blocks run at once (clusters of 4 and 8 leave SMs
-// unused).  Its constants are fitted to 746 measured plans of 54 shapes (m 1 .. 3986, k 32 .. 11008, n 16 .. 11008, both layouts): the
-// chosen plan takes 0.4 % longer than the best on average, 6 % at worst.  Among them: 1 x 4096 x 11008 split 4, 16 tokens 11.4 us,
-// unsplit 13.4; 200 x 4096 x 11008 in pairs 17.3, else 18.4; 200 x 11008 x 4096 split 4, 128 tokens 19.7, in pairs 33; 1000 x 4096
-// x 11008 in pairs of 224 tokens 38.8, of 256 39, of 128 58, single blocks 57.
+// come from HBM (5.4 MB a us, to pairs 6.3 MB); of single blocks the operand bytes of all tiles on their way to the busiest SM (one
+// block's at 61 KB a us, several blocks' together at 91 KB) or its products, 1850 columns a us; of pairs a slice's time, 0.18 us
+// and 0.10 us for 256 tokens, or the write-out; a fixed part for set-up and end, the last write-out, rounds, the barriers of a
+// split, and how many blocks run at once (clusters of 4 and 8 leave SMs unused).  Its constants are fitted to 1145 measured plans
+// of 76 shapes (m 1 .. 3986, k 32 .. 11008, n 16 .. 32000, both layouts): 16 % off where a plan is not far from the best, and the
+// chosen plan takes 1.5 % longer than the best on average, 21 % at worst (932 x 704 x 48, 7.2 us).  Among them (us): 16 x 4096 x
+// 11008 split 4 11.6, unsplit 14.7, in pairs 11.5; 200 x 4096 x 11008 in pairs 15.3, else 17.2; 200 x 11008 x 4096 split 4 of 128
+// tokens 19.1, in pairs 22.6; 1000 x 4096 x 11008 in pairs of 224 tokens 35.7, of 256 36.0, of 128 42, single blocks 48.5.  A pair
+// makes 32 tokens at least, so up to 16 tokens go to single blocks (1 x 4096 x 11008 11.1 / 11.7, 1 x 4096 x 4096 6.9 / 10.6,
+// 1 x 4096 x 32000 24.1 / 23.5).
 //
 // `off_grid`: bytes of the operands that TMA cannot read in place.  They are copied first (4.7 MB a us, read and written, and a
 // launch more: 4 us, most of it the host's), or, where a tile has few slices, shifted on their way: about 4.4 us for a block's first
@@ -581,7 +585,7 @@ inline int blocks_at_once(int split, int room) { return (split <= 2 ? 148 : spli
 // 16 x 11007 x 4095 31 / 25, 100 x 4095 x 11007 36 / 64).
 Plan make_plan(int m, int k, int n, int64_t off_grid) {
     const int slices = (k + I8_KS - 1) / I8_KS, n128 = (n + 127) / 128, n256 = (n + 255) / 256;
-    const float hbm = ((float)k * n + (float)m * k + 2.0f * m * n) / 6.14e6f;
+    const float from_hbm = (float)k * n + (float)m * k + 2.0f * m * n, hbm = from_hbm / 5.44e6f, hbm_pairs = from_hbm / 6.26e6f;
     Plan best = {};
     float least = 1e30f;
     static const int widths[] = {16, 32, 48, 64, 96, 128, 192, 256};
@@ -593,19 +597,20 @@ Plan make_plan(int m, int k, int n, int64_t off_grid) {
             const int ctas = tiles * split, steps = (slices + split - 1) / split;
             const int spread = blocks_at_once(split, 1), rounds = (ctas + spread * room - 1) / (spread * room);
             const float bytes = i8_stage_bytes(nt), product = nt / 1850.0f;
-            const float sm = (float)((ctas + spread - 1) / spread) * steps * std::max(bytes / 77e3f, product);
-            const float alone = (float)rounds * steps * std::max(bytes / 50e3f, product);
-            const float t = 2.85f + std::max(hbm, std::max(sm, alone)) + 4.0f * nt / 256 / split * rounds + (split > 1 ? 0.6f : 0.0f) + (rounds - 1);
+            const float sm = (float)((ctas + spread - 1) / spread) * steps * std::max(bytes / 91.3e3f, product);
+            const float alone = (float)rounds * steps * std::max(bytes / 60.9e3f, product);
+            const float t = 2.71f + std::max(hbm, std::max(sm, alone)) + 2.79f * nt / 256 / split * rounds + (split > 1 ? 1.42f : 0.0f) + 2.28f * (rounds - 1);
             if (t < least) {
                 least = t;
                 best = {false, false, nt, split, (room == 3 ? 70 : room == 2 ? 104 : 200) * 1024 / i8_stage_bytes(nt)};
             }
         }
     }
-    for (int nt = 32; nt <= 256 && (nt == 32 || nt < m + 32); nt += 32) {
+    for (int nt = 32; nt <= 256 && m > 16 && (nt == 32 || nt < m + 32); nt += 32) {
         const int64_t tiles = (int64_t)((m + nt - 1) / nt) * n256;
         const float per = (float)((tiles + 73) / 74);
-        const float t = 1.9f + std::max(hbm, per * slices * std::max((16384 + 64 * nt) / 59.4e3f, nt / 925.0f)) + 1.8f * nt / 256;
+        const float part = nt / 256.0f;
+        const float t = 3.44f + std::max(hbm_pairs, per * std::max(slices * (0.179f + 0.104f * part), 2.39f * part)) + 3.05f * part + 1.03f * (per - 1);
         if (t < least) {
             least = t;
             best = {true, false, nt, 1, std::min(I8_PAIR_STAGES, 200 * 1024 / i8_pair_stage_bytes(nt))};
