@@ -8,11 +8,14 @@
 // (vocab / 64 of a row of 1024 packs or less), two by two.
 //
 // Alternatives without a second pass: a thread's packs (the entries of one 16-byte load) fall into four shares, and it keeps
-// the largest entry of each share and the pack that first reached it.  The threads form 64 groups (32 for up to 16
-// alternatives: 4096 x 32000 bf16 with 5 57.0 -> 55.7 us), each with the best (value, pack) of its shares as key; a pack belongs to one share, so keys are distinct.  An entry that is among the `top` best lies
-// in a share whose own key is at least the top-th largest group key: were it smaller, the `top` entries behind those keys
-// would all come before it.  Only those shares, a few hundred entries of a row, are read again (from L2), what is not below
-// the key is collected and ranked by counting.
+// the largest entry of each share and the pack that first reached it.  The threads form 64 groups (32 for up to 16 alternatives:
+// 4096 x 32000 bf16 with 5 57.0 -> 55.7 us), each with the best (value, pack) of its shares as key; a pack belongs to one share,
+// so keys are distinct.  An entry that is among the `top` best lies in a share whose own key is at least the top-th largest group
+// key: were it smaller, the `top` entries behind those keys would all come before it.  Only those shares, a few hundred entries
+// of a row, are read again (from L2), what is not below the key is collected and ranked by counting.
+//
+// Bound by HBM where rows are many: 4096 x 32000 bf16 without a list 49 us, 5 us of start and then 6.0 TB/s; the list's instructions
+// come on top.  Few rows are latency: the loads of a thread, the joins of a block and of a cluster.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
