@@ -14,6 +14,7 @@ __device__ __forceinline__ void await_inputs() { asm volatile("griddepcontrol.wa
 // are done: earlier, the next kernel's blocks would take the room that is free at the moment and lie unevenly on the SMs.
 __device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// `cluster` blocks to a cluster; without `early` the kernel starts when those before it have ended.
 template <typename... Params, typename... Args>
 int launch_early(const char* what, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, bool early, cudaStream_t st, Args... args) {
     cudaLaunchAttribute attr[2];
