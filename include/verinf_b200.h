@@ -341,7 +341,8 @@ int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_
  * where that would take longer, first copied to the scratch: vi_int8_matmul_scratch_bytes (0 where nothing is copied),
  * 16-byte aligned.  Whole 16-byte cells are read, bytes beside a row that lie in its first and last cell among them.
  * vi_int8_matmul_status: *code = non-zero if a product on the current device gave up on one of its bounded waits since the
- * last call (its output is then incomplete); waits for the device. */
+ * last call (its output is then incomplete); waits for all streams of the device first, so it is not called while one is
+ * captured. */
 int64_t vi_int8_matmul_scratch_bytes(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel,
                                      int64_t m, int64_t k, int64_t n);
 int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_by_channel,

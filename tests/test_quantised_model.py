@@ -783,3 +783,21 @@ def test_quantised_head_workload():
     root, _, _ = cp.commit_rows(rows, w.K_DEG, w.N_LIG, master_seed=torch.arange(32, dtype=torch.uint8, device=dev))
     assert bytes(root.cpu().tolist()).hex() == out["root"]
     assert 0 < out["mean_entropy_bits"] < math.log2(1000) and out["mean_bits"] > 0
+
+
+@gpu
+def test_errors_are_asked_for_behind_every_stream(i8):
+    """A product on a side stream that is still waiting to run has ended when its errors have been asked for."""
+    g = torch.Generator().manual_seed(14)
+    A, B = _rand8(g, 32, 1024).cuda(), _weight(g, 1024, 512, "nk", 0)
+    i8.int8_matmul(A, B)
+    side, ended = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)              # about a tenth of a second
+        y = i8.int8_matmul(A, B)
+        ended.record()
+    assert not ended.query()
+    i8.check_async_errors()
+    assert ended.query()
+    assert torch.equal(y.cpu().long(), _sums_64(A, B))

@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 #include "../../include/verinf_b200.h"
 #include "common.cuh"
@@ -36,7 +37,8 @@ constexpr int I8_TN = 128, I8_KS = 128, I8_THREADS = 256, I8_MAX_STAGES = 8, I8_
 constexpr int I8_W_BYTES = I8_TN * I8_KS;
 constexpr int I8_TAIL = 2 * I8_MAX_STAGES * 8 + 64 + 256 * 4;      // barriers, tensor-memory slot, scales of the tokens
 
-__device__ int g_i8_status;                                          // first wait that expired, 0 = none
+__device__ int g_i8_status, g_i8_taken;                              // first wait that expired, 0 = none; what the last question took
+__global__ void k_int8_take_status() { g_i8_taken = atomicExch(&g_i8_status, 0); }
 
 struct Plan { bool pair, direct; int nt, split, stages; };
 __host__ __device__ inline int i8_stage_bytes(int nt) { return I8_W_BYTES + nt * I8_KS; }
@@ -744,10 +746,16 @@ extern "C" int vi_int8_matmul(const int8_t* A, int64_t lda, const int8_t* B, int
     }
 }
 
+// The device is waited for first: the legacy default stream, on which the copy runs, does not wait for non-blocking streams.  Read
+// and cleared in one step, so that a code that a product of another host thread records meanwhile is kept for the next call.
 extern "C" int vi_int8_matmul_status(int* code) {
     VI_REQUIRE(code, "int8_matmul_status: null pointer");
-    const int none = 0;
-    VI_CUDA(cudaMemcpyFromSymbol(code, g_i8_status, sizeof(int)));
-    if (*code) VI_CUDA(cudaMemcpyToSymbol(g_i8_status, &none, sizeof(int)));
+    static std::mutex one;              // g_i8_taken is this call's until it is read
+    std::lock_guard<std::mutex> lock(one);
+    VI_CUDA(cudaDeviceSynchronize());
+    k_int8_take_status<<<1, 1>>>();
+    const int rc = vi::check_launch("k_int8_take_status");
+    if (rc) return rc;
+    VI_CUDA(cudaMemcpyFromSymbol(code, g_i8_taken, sizeof(int)));
     return VI_OK;
 }

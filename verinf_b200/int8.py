@@ -154,7 +154,7 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
 
 def check_async_errors(device=None):
     """Raises if a product launched earlier on the device gave up on one of its bounded device-side waits (its output is then
-    incomplete).  Waits for the device."""
+    incomplete).  Waits for all streams of the device, so it is not called while one is captured."""
     code = C.c_int(0)
     with torch.cuda.device(device):
         check(LIB.vi_int8_matmul_status(C.byref(code)))
