@@ -801,3 +801,27 @@ def test_errors_are_asked_for_behind_every_stream(i8):
     i8.check_async_errors()
     assert ended.query()
     assert torch.equal(y.cpu().long(), _sums_64(A, B))
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1.0, 2.5, 1000.0, 1e6])
+def test_logprobs_of_values_far_apart(lp, temperature):
+    """fp32 values whose difference is beyond fp32, while that over the temperature is not: likely and unlikely tokens, short rows and
+    rows of a cluster."""
+    most = torch.finfo(torch.float32).max
+    for vocab in (5, 70001):
+        x = torch.full((6, vocab), -math.inf)
+        x[:, :5] = torch.tensor([[most, -most, -most / 2, 0.0, 1.0], [-most, most, most, -0.75 * most, -math.inf], [-most] * 5,
+                                 [-most, 3.0, 2.5, 2.0, -math.inf], [2e38, -2e38, -1.5e38, 1.5e38, 1.9e38],
+                                 [-most, -most / 2, -math.inf, -math.inf, -math.inf]])
+        tokens = torch.tensor([1, 0, 3, 0, 1, 0])
+        out = lp.token_logprobs(x.cuda(), tokens.cuda(), top=5, temperature=temperature)
+        want = _logprobs_64(x, tokens, 5, temperature)
+        # of ln p: the difference, 1 / T, their product and the difference with the logarithm of the sum, half a step each, and what
+        # these four make together; the sum itself as in _check_logprobs, its constant rounded too
+        u = HALF[torch.float32]
+        rel = (5 * 24 + 4 + vocab / 256 + 64) * u
+        assert torch.equal(out.top_token.cpu(), want[3])
+        for got, w in ((out.logprob, want[0]), (out.top_logprob, want[2])):
+            assert _near(got, w, rel + u * (8 * want[4].reshape([-1] + [1] * (w.dim() - 1)) + 5 * torch.nan_to_num(w, 0, 0, 0).abs()))
+        assert _near(out.entropy, want[1], rel * (1 + 2 * want[5]) + 8 * u * (want[4] + want[5]))

@@ -121,11 +121,12 @@ struct Stat { float m, s, w; };      // max, sum 2^a, sum 2^a a
 // its rounding, at most 2^-4 where |m c| < 2^20, cancels between a_t and log2 S.  Elsewhere the difference comes first.
 __device__ __forceinline__ bool is_near(float m, float c) { return fabsf(__fmul_rn(m, c)) < LP_FAR; }
 __device__ __forceinline__ float arg_of(float x, float m, float c) { return is_near(m, c) ? __fmaf_rn(x, c, -__fmul_rn(m, c)) : (x - m) * c; }
-// ln p of an entry.  Where the product with c could overflow though the difference over T does not, that comes first; no
-// rounding makes a probability larger than one.
+// ln p of an entry.  Where the product with c could overflow though the difference over T does not, the difference comes first, of
+// halves, which does not overflow either (a half that is not exact, of a subnormal number, has |m| >= 2^20 / c > 0.7 or an x
+// below LP_CLAMP beside it, and does not count); no rounding makes a probability larger than one.
 __device__ __forceinline__ float log_p(float x, const Stat& all, float c, float inv_t, float log_s) {
     const float ln2 = 0.6931471805599453f;
-    const float v = is_near(all.m, c) && x > LP_CLAMP ? (arg_of(x, all.m, c) - log_s) * ln2 : (x - all.m) * inv_t - log_s * ln2;
+    const float v = is_near(all.m, c) && x > LP_CLAMP ? (arg_of(x, all.m, c) - log_s) * ln2 : (0.5f * x - 0.5f * all.m) * (2.0f * inv_t) - log_s * ln2;
     return fminf(v, 0.0f);
 }
 // what a grows by when the maximum goes from `from` to `to`: the rounded m c is the reference of a short form, the exact one of
