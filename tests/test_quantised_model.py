@@ -3,6 +3,9 @@ bits; what they refuse; a run of them together.  Tolerances are counted in round
 fp32, 2^-11 in fp16, 2^-8 in bf16."""
 import ctypes as C
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -825,3 +828,42 @@ def test_logprobs_of_values_far_apart(lp, temperature):
         for got, w in ((out.logprob, want[0]), (out.top_logprob, want[2])):
             assert _near(got, w, rel + u * (8 * want[4].reshape([-1] + [1] * (w.dim() - 1)) + 5 * torch.nan_to_num(w, 0, 0, 0).abs()))
         assert _near(out.entropy, want[1], rel * (1 + 2 * want[5]) + 8 * u * (want[4] + want[5]))
+
+
+def test_import_without_torchs_short_calls():
+    """A torch that lacks the calls which the entry points prefer has the public ones, and the package imports."""
+    prog = """
+import torch
+hidden = []
+for place, name in ((torch._C, "_cuda_getDevice"), (torch._C, "_cuda_getCurrentRawStream"), (torch._C._dynamo.guards, "_empty_strided_cuda")):
+    if hasattr(place, name):
+        hidden.append((place, name, getattr(place, name)))
+        delattr(place, name)
+from verinf_b200 import _lib, int8, logprobs
+for place, name, call in hidden:                 # the public calls may use them
+    assert call not in (_lib.current_device, _lib.raw_stream, _lib.empty_strided)
+    setattr(place, name, call)
+try:
+    int8.int8_quantize_rows(torch.zeros(2, 3))
+except RuntimeError as e:
+    assert "CUDA" in str(e)
+if torch.cuda.is_available():
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert _lib.raw_stream(0) == side.cuda_stream and _lib.current_device() == 0
+        x = torch.tensor([[1.0, -2.0]], device="cuda")
+        q, s = int8.int8_quantize_rows(x)
+        assert q.tolist() == [[64, -127]]
+        assert int8.int8_matmul(q, q.t()).item() == 64 * 64 + 127 * 127
+        assert logprobs.token_logprobs(x, torch.tensor([0], device="cuda"), top=1).top_token.item() == 0
+print("imported")
+"""
+    root = Path(__file__).resolve().parents[1]
+    out = subprocess.run([sys.executable, "-c", prog], cwd=root, capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0 and out.stdout.strip() == "imported", out.stderr[-2000:]
+
+
+@gpu
+def test_torchs_public_calls_do_as_well():
+    """The same on the GPU: the kernels run on the current stream that the public calls name."""
+    test_import_without_torchs_short_calls()

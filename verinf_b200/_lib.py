@@ -114,8 +114,16 @@ def stream_ptr() -> int:
 # torch's current stream of a device index as a number, and an uninitialised tensor (shape, strides, dtype) on the current device,
 # by the calls that torch's own generated code makes: 0.1 us instead of 2.2 us for torch.cuda.current_stream, 0.8 us instead of
 # 2.4 us for torch.empty, of the 10 us that a small call takes.
-current_device = torch._C._cuda_getDevice
-raw_stream = torch._C._cuda_getCurrentRawStream
+# The public calls stand in where a torch lacks them (a build without CUDA, another release).
+try:
+    current_device = torch._C._cuda_getDevice
+except AttributeError:
+    current_device = torch.cuda.current_device
+try:
+    raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 try:
     empty_strided = torch._C._dynamo.guards._empty_strided_cuda
 except AttributeError:
