@@ -867,3 +867,24 @@ print("imported")
 def test_torchs_public_calls_do_as_well():
     """The same on the GPU: the kernels run on the current stream that the public calls name."""
     test_import_without_torchs_short_calls()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("vocab", [3, 2999])
+def test_logprobs_the_token_comes_before_the_row(lp, dtype, vocab):
+    """No token and a token outside the vocabulary beside rows with a NaN, with +inf, of -inf alone and ordinary ones; entropy says
+    which rows are valid."""
+    rows = torch.zeros(4, vocab)
+    rows[0, vocab - 1], rows[1, 0], rows[2] = math.nan, math.inf, -math.inf
+    tokens = torch.tensor([-1, -(1 << 62), vocab, (1 << 40) + 1, 1])
+    out = lp.token_logprobs(rows.repeat(5, 1).to(dtype).cuda(), tokens.repeat_interleave(4).cuda(), top=2)
+    logprob, entropy = out.logprob.cpu().view(5, 4), out.entropy.cpu().view(5, 4)
+    # equal entries: the sum, its logarithm and the difference, counted as in _check_logprobs
+    tol = (4 + vocab / 256 + 64 + 12 * math.log(vocab)) * HALF[torch.float32]
+    assert (logprob[:2] == 0).all() and torch.isnan(logprob[2:4]).all()
+    assert torch.isnan(logprob[4, :2]).all() and logprob[4, 2] == -math.inf and abs(logprob[4, 3] + math.log(vocab)) < tol
+    assert torch.isnan(entropy[:, :2]).all() and (entropy[:, 2] == 0).all() and ((entropy[:, 3] - math.log(vocab)).abs() < tol).all()
+    lists, ids = out.top_logprob.cpu().view(5, 4, 2), out.top_token.cpu().view(5, 4, 2)
+    assert torch.isnan(lists[:, :2]).all() and (lists[:, 2] == -math.inf).all() and (ids[:, :3] == -1).all()
+    assert (ids[:, 3] == torch.tensor([0, 1])).all()
