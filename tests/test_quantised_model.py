@@ -888,3 +888,76 @@ def test_logprobs_the_token_comes_before_the_row(lp, dtype, vocab):
     lists, ids = out.top_logprob.cpu().view(5, 4, 2), out.top_token.cpu().view(5, 4, 2)
     assert torch.isnan(lists[:, :2]).all() and (lists[:, 2] == -math.inf).all() and (ids[:, :3] == -1).all()
     assert (ids[:, 3] == torch.tensor([0, 1])).all()
+
+
+# ---- many rows: a block of 64 or 128 threads a row -------------------------------------------------------------------------
+def _logprobs_rows_64(x, tokens, top, temperature):
+    """What _logprobs_64 gives, for all rows at once (where x is)."""
+    x = x.double() + 0.0                                             # -0 counts as 0
+    rows, vocab = x.shape
+    bad, none = (torch.isnan(x) | (x == math.inf)).any(1), (x == -math.inf).all(1)
+    x = torch.where(bad[:, None], 0.0, x)
+    z = (x - torch.where(none[:, None], 0.0, x.amax(1, keepdim=True))) / temperature
+    e = z.exp()
+    s = torch.where(none, 1.0, e.sum(1))
+    log_z, width = s.log(), -(e * torch.where(e > 0, z, 0.0)).sum(1) / s
+    ent = torch.where(bad, math.nan, log_z + width)
+    lp = z.gather(1, tokens.clamp(0, vocab - 1)[:, None])[:, 0] - log_z
+    lp = torch.where(tokens < 0, 0.0, torch.where((tokens >= vocab) | bad, math.nan, lp))
+    tt = x.sort(dim=1, descending=True, stable=True)[1][:, :top]
+    tl = z.gather(1, tt) - log_z[:, None]
+    tt = torch.where((tl == -math.inf) | bad[:, None], -1, tt)
+    tl = torch.where(bad[:, None], math.nan, tl)
+    short = top - tt.size(1)                                         # fewer entries than the list holds
+    if short > 0:
+        tt = torch.cat([tt, tt.new_full((rows, short), -1)], 1)
+        tl = torch.cat([tl, torch.where(bad[:, None], math.nan, -math.inf).double().expand(rows, short)], 1)
+    return lp, ent, tl, tt, log_z, width
+
+
+def _check_many_rows(lp_mod, x, tokens, tops, temperature):
+    lp, ent, tl, tt, log_z, width = _logprobs_rows_64(x, tokens, 32, temperature)
+    # as in _check_logprobs, with a rounded 1 / T (two half steps more of a difference) and the longest chain, that of 64 threads
+    u = HALF[torch.float32]
+    rel = (5 * 24 + 4 + x.size(1) / 64 + 64) * u
+    t = lambda want, steps: (rel + u * (8 * log_z.reshape([-1] + [1] * (want.dim() - 1)) + steps * torch.nan_to_num(want, 0, 0, 0).abs())).cpu()
+    for top in tops:
+        out = lp_mod.token_logprobs(x, tokens, top=top, temperature=temperature)
+        assert torch.equal(out.top_token, tt[:, :top])
+        assert _near(out.logprob, lp.cpu(), t(lp, 6))
+        assert _near(out.entropy, ent.cpu(), (rel * (1 + 2 * width) + 8 * u * (log_z + width)).cpu())
+        assert _near(out.top_logprob, tl[:, :top].cpu(), t(tl[:, :top], 6))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,vocab,offset,pitch,masked,temperature",
+                         [(512, 1, 0, 1, "no", 1.0), (513, 31, 0, 31, "no", 0.7), (2000, 300, 1, 305, "inf", 1.0), (515, 4001, 0, 4001, "lowest", 1.5),
+                          (700, 4096, 0, 4096, "no", 1.0), (600, 8200, 3, 8209, "inf", 0.7), (1100, 9001, 0, 9008, "lowest", 1.0),
+                          (520, 33000, 0, 33000, "no", 1.0), (516, 32001, 5, 32011, "inf", 1.3)])
+def test_logprobs_many_rows(lp, dtype, rows, vocab, offset, pitch, masked, temperature):
+    """Every row against 64 bits, lists on both sides of the change of the number of groups; rows that are masked in part or whole,
+    hold fewer entries than the list, equal ones, a NaN or infinity, or crowd their large entries in a few threads' shares."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    x = torch.randn(rows, vocab, device="cuda", generator=g) * 3
+    x.scatter_add_(1, torch.randint(0, vocab, (rows, 12), device="cuda", generator=g), torch.rand(rows, 12, device="cuda", generator=g) * 9)
+    low = torch.finfo(dtype).min if masked == "lowest" else -math.inf
+    if masked != "no":
+        x[torch.rand(rows, vocab, device="cuda", generator=g) < 0.4] = low
+    i = torch.arange(vocab, device="cuda")
+    x[3] = low
+    x[4, vocab // 2] = math.nan
+    x[5, vocab - 1] = math.inf
+    x[6] = 1.25
+    x[7] = torch.where(i % 2 == 0, 0.0, -0.0)
+    x[8] = torch.where(i % max(1, vocab // 7) == 0, 2.0 + 0.25 * (i % 5), -math.inf)
+    x[9] = torch.linspace(-9, 9, vocab, device="cuda")
+    x[10] = torch.linspace(9, -9, vocab, device="cuda")
+    for r, step in ((11, 512), (12, 1024), (13, 2048)):
+        x[r] = torch.where(i % step < 16, (i // step).float() / 64 + i % 16, -math.inf)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    tokens[20], tokens[21], tokens[rows - 1] = -1, vocab, 0
+    buf = torch.full((rows, pitch + offset), 100.0, dtype=dtype, device="cuda")       # behind the vocabulary: not part of it
+    view = buf[:, offset:offset + vocab]
+    view.copy_(x.to(dtype))
+    _check_many_rows(lp, view, tokens, (0, 1, 5, 16, 17, 32), temperature)
