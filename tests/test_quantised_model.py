@@ -961,3 +961,99 @@ def test_logprobs_many_rows(lp, dtype, rows, vocab, offset, pitch, masked, tempe
     view = buf[:, offset:offset + vocab]
     view.copy_(x.to(dtype))
     _check_many_rows(lp, view, tokens, (0, 1, 5, 16, 17, 32), temperature)
+
+
+# ---- operands that are copied first ------------------------------------------------------------------------------------
+def _scratch_bytes(i8, lib, A, B):
+    """What int8_matmul asks for these operands."""
+    m, k, lda = i8.matrix(A, "", "A", (torch.int8,))
+    B, k, n, by_channel, ldb = i8._weight(B, "")
+    return lib.LIB.vi_int8_matmul_scratch_bytes(A.data_ptr(), lda, B.data_ptr(), ldb, by_channel, m, k, n)
+
+
+def _laid(g, rows, cols, offset, pitch):
+    """rows x cols int8 on the GPU whose first entry is `offset` bytes behind the 16-byte grid, rows `pitch` bytes apart."""
+    buf = _rand8(g, rows * pitch + 32).cuda()
+    assert buf.data_ptr() % 16 == 0 and pitch >= cols
+    return torch.as_strided(buf, (rows, cols), (pitch, 1), offset)
+
+
+def _on_grid(n):
+    return (n + 15) // 16 * 16
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("off", ["A", "B", "both"])
+@pytest.mark.parametrize("m,k,n", [(120, 4001, 1003), (300, 2001, 1500), (700, 3001, 2001), (256, 1203, 2001)])
+def test_matmul_copied_operands(i8, lib, layout, off, m, k, n):
+    """One operand or both off the 16-byte grid, by their rows' distance or their first byte, at sizes where they are copied; then
+    clusters, single blocks and pairs make the product.  On the grid, nothing is asked for."""
+    g = torch.Generator().manual_seed(m + k + n)
+    rows, cols = (k, n) if layout == "kn" else (n, k)
+
+    def operands(offset, a_pitch, b_pitch):
+        b = _laid(g, rows, cols, offset if off != "A" else 0, b_pitch if off != "A" else _on_grid(cols))
+        return _laid(g, m, k, offset if off != "B" else 0, a_pitch if off != "B" else _on_grid(k)), b if layout == "kn" else b.t()
+
+    for offset, a_pitch, b_pitch in [(0, k, cols), (1, _on_grid(k), _on_grid(cols)), (15, _on_grid(k), _on_grid(cols) + 16), (7, k + 2, cols + 6)]:
+        A, B = operands(offset, a_pitch, b_pitch)
+        assert _scratch_bytes(i8, lib, A, B) >= (m * k if off != "B" else 0) + (k * n if off != "A" else 0)
+        _check_matmul(i8, A, B, [torch.int32, torch.uint64, torch.bfloat16], g, out_pad=3)
+    A, B = operands(0, _on_grid(k), _on_grid(cols))
+    assert _scratch_bytes(i8, lib, A, B) == 0
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("m,k,n", [(1, 515, 1001), (5, 515, 1001), (31, 515, 1001), (17, 515, 3001), (700, 515, 301)])
+def test_matmul_copied_tokens_alone(i8, lib, layout, m, k, n):
+    """Few tokens off the grid beside a weight on it: copied, and the product made by single blocks."""
+    g = torch.Generator().manual_seed(m + k + n)
+    rows, cols = (k, n) if layout == "kn" else (n, k)
+    for offset, pitch in [(1, _on_grid(k)), (8, k), (15, k + 10)]:
+        A, b = _laid(g, m, k, offset, pitch), _laid(g, rows, cols, 0, _on_grid(cols))
+        B = b if layout == "kn" else b.t()
+        assert _scratch_bytes(i8, lib, A, B) == m * _on_grid(k)
+        _check_matmul(i8, A, B, g=g)
+
+
+@gpu
+def test_two_streams_and_two_graphs_with_copies(i8, lib):
+    """Products whose operands are copied first, on two streams at once and in two captured graphs replayed in turn and at once: each
+    call has copies of its own."""
+    g = torch.Generator().manual_seed(16)
+    shapes = [(300, 2001, 1501, "kn"), (120, 4001, 1003, "nk")]
+    A = [_rand8(g, m, k).cuda() for m, k, n, _ in shapes]
+    B = [_weight(g, k, n, layout, 0) for m, k, n, layout in shapes]
+    for a, b in zip(A, B):
+        assert _scratch_bytes(i8, lib, a, b) >= a.numel() + b.numel()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(8):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                results[j].append(i8.int8_matmul(A[j], B[j]))
+                results[j].append(i8.int8_matmul(A[j].neg(), B[j]))       # another operand into the room that is free again
+    torch.cuda.synchronize()
+    for j in range(2):
+        S, N = _sums_64(A[j], B[j]), _sums_64(A[j].neg(), B[j])
+        assert all(torch.equal(y.cpu().long(), (S, N)[i % 2]) for i, y in enumerate(results[j]))
+    graphs, outs = [], []
+    for j in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(i8.int8_matmul(A[j], B[j]))
+        graphs.append(graph)
+    for _ in range(3):
+        graphs[0].replay()
+        streams[0].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[0]):
+            graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for j in range(2):
+            assert torch.equal(outs[j].cpu().long(), _sums_64(A[j], B[j]))
+            A[j].copy_(_rand8(g, *A[j].shape))
+            B[j].copy_(_rand8(g, *B[j].shape))
