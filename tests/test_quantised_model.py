@@ -1057,3 +1057,27 @@ def test_two_streams_and_two_graphs_with_copies(i8, lib):
             assert torch.equal(outs[j].cpu().long(), _sums_64(A[j], B[j]))
             A[j].copy_(_rand8(g, *A[j].shape))
             B[j].copy_(_rand8(g, *B[j].shape))
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("m,k,n", [(1001, 1200, 20000), (2001, 304, 9008), (4095, 128, 5008), (515, 2064, 30000), (777, 1040, 32000)])
+def test_matmul_many_tiles_a_pair(i8, layout, m, k, n):
+    """More tiles than three rounds of 74 pairs of blocks even at the largest tile of 256 x 256, and numbers of slices that no ring of 6, 7 or 8
+    stages divides evenly: both accumulators, the wait for one that is written out, and a ring that goes on from tile to tile.  The whole
+    result, with remainders of every size."""
+    assert -(-m // 256) * -(-n // 256) > 3 * 74
+    g = torch.Generator().manual_seed(m + k + n)
+    A, B = _rand8(g, m, k).cuda(), _weight(g, k, n, layout, 0)
+    S = (A.double() @ B.double()).to(torch.int64)                    # whole in 64 bits
+    assert torch.equal(i8.int8_matmul(A, B), S.to(torch.int32))
+    lifted = torch.where(S < 0, S + (P - (1 << 64)), S)
+    assert torch.equal(i8.int8_matmul(A, B, dtype=torch.uint64).view(torch.int64), lifted)
+    sa, sb = torch.rand(m, generator=g).cuda() + 0.01, torch.rand(n, generator=g).cuda() * 1e-3
+    want = S.double() * sa.double()[:, None] * sb.double()
+    for dtype in (torch.float32, torch.bfloat16):
+        y = i8.int8_matmul(A, B, sa, sb, dtype=dtype).double()
+        # roundings: the sum to fp32, two products, the output type where it is shorter
+        tol = want.abs() * (3 * HALF[torch.float32] + (HALF[dtype] if dtype != torch.float32 else 0)) * 1.001 + 1e-37
+        assert ((y - want).abs() <= tol).all()
+    i8.check_async_errors()
