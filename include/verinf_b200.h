@@ -328,7 +328,7 @@ enum { VI_F32 = 0, VI_F16 = 1, VI_BF16 = 2, VI_I32 = 3, VI_FIELD = 4 };
 /* Rows to int8 with one scale a row: x (m, k) of VI_F32 / VI_F16 / VI_BF16, rows x_stride elements apart (0: the same row);
  * scale[r] = max_j |x_rj| / 127, q_rj = the whole number nearest to 127 x_rj / max_j |x_rj| (of the exact quotient, ties
  * to even), in rows q_stride bytes apart.  A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN and
- * q = 0. */
+ * q = 0.  x, q and scale share no memory: a long row is read twice, after parts of it are written. */
 int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t x_stride,
                           int8_t* q, int64_t q_stride, float* scale, void* stream);
 
@@ -336,7 +336,7 @@ int vi_int8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_
  * apart, or, with b_by_channel, stored (n, k) with the k values of a channel together and channels ldb bytes apart.
  * out_type VI_F32 / VI_F16 / VI_BF16: C_ij = (S_ij * sa_i) * sb_j in fp32, rounded once to the type (sa (m), sb (n); NULL =
  * ones); VI_I32: S; VI_FIELD: S mod p as uint64_t, negative sums as p - |S| (the same value vi_gl_matmul gives for the
- * lifted operands); these two take no scales.  C rows ldc elements apart; C must not overlap an operand.
+ * lifted operands); these two take no scales.  C rows ldc elements apart; C must not overlap an operand or the scales.
  * Operands whose rows (channels) all start on 16-byte boundaries are read in place; others are shifted on their way, or,
  * where that would take longer, first copied to the scratch: vi_int8_matmul_scratch_bytes (0 where nothing is copied),
  * 16-byte aligned.  Whole 16-byte cells are read, bytes beside a row that lie in its first and last cell among them.

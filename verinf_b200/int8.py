@@ -59,7 +59,7 @@ def int8_quantize_rows(x, out=None):
     scale[r] = max_j |x[r, j]| / 127 and q[r, j] = the whole number nearest to 127 x[r, j] / max_j |x[r, j]|, ties to even: of
     the exact quotient, so that whoever quantises the same row gets the same whole numbers.  A row of zeros has scale 0; one
     that holds a NaN or an infinity has scale NaN and zeros.  `out`: a pair (q, scale) to write into; the rows of q may be any
-    distance apart."""
+    distance apart; neither shares memory with x or the other (a long row is read twice, after parts of it are written)."""
     index = x.get_device() if isinstance(x, torch.Tensor) else -1
     if index >= 0 and index != current_device():
         with torch.cuda.device(index):
@@ -113,7 +113,7 @@ def int8_matmul(A, B, scale_a=None, scale_b=None, dtype=torch.int32, out=None):
     The rows of A may be any distance apart.  B is row-major with rows any distance apart, or the transposed view of a weight
     stored by output channel (`weight.t()`), its channels any distance apart.  Rows (channels) that start on 16-byte
     boundaries are fastest; others are shifted on their way or copied, on every call.  `out`: a tensor of `dtype` to write
-    into, rows any distance apart; it must not share memory with the operands."""
+    into, rows any distance apart; it must not share memory with the operands or the scales."""
     index = A.get_device() if isinstance(A, torch.Tensor) else -1
     if index >= 0 and index != current_device():
         with torch.cuda.device(index):
