@@ -357,7 +357,9 @@ int vi_int8_matmul_status(int* code);
  * -inf are tokens that are not allowed; where fewer than `top` are left, the rest of the list is -1 with -inf.  A row of
  * nothing but -inf has logprob -inf and entropy 0; one that holds a NaN or +inf has NaN in all its numbers and an empty
  * list (top_token -1).  The token comes before the row: logprob is 0 for a negative token and NaN for one of vocab or more,
- * whatever the row holds, so entropy tells whether a row is valid.  1e-6 <= temperature <= 1e6. */
+ * whatever the row holds, so entropy tells whether a row is valid.  Sums are in fp32, in an order that follows rows, vocab and
+ * where a row starts: the same call gives the same bits, a row alone and the row in a batch may differ in the last ones (not in
+ * top_token).  1e-6 <= temperature <= 1e6. */
 int vi_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
                       const int64_t* tokens, int top, double temperature,
                       float* logprob, float* entropy, float* top_logprob, int64_t* top_token, void* stream);

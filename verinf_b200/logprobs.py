@@ -29,7 +29,11 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     An entry of -inf is a token that is not allowed; a list with fewer allowed tokens than `top` ends in -1 and -inf.  A row of
     -inf alone has logprob -inf, entropy 0 and an empty list.  A row with a NaN or +inf has NaN in its numbers and an empty
     list (-1).  The token comes before the row: logprob is 0 for a negative token and NaN for one >= vocab whatever the row holds, so
-    look for rows that are not valid in entropy.  Returns a TokenLogprobs, which carries no gradient."""
+    look for rows that are not valid in entropy.
+
+    The sums are in fp32, in an order that follows the number of rows in the call, the vocabulary and where a row starts: the same
+    call gives the same bits, but a row's numbers in a batch may differ in their last bits from those of the row alone (top_token does
+    not).  Returns a TokenLogprobs, which carries no gradient."""
     index = logits.get_device() if isinstance(logits, torch.Tensor) else -1
     if index >= 0 and index != current_device():
         with torch.cuda.device(index):
