@@ -156,8 +156,10 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
 enum { I8_ERR_FULL = 1, I8_ERR_EMPTY = 2, I8_ERR_ACC = 3 };
 
 // One tile a block, or, with split > 1, one tile a cluster whose blocks each take a share of the terms; the sums meet through
-// distributed shared memory (whole numbers: the order does not matter).  For few tokens, where the weight's bytes and the latency
-// of the first loads and of the join bind: 1 x 4096 x 11008 10.6 us (4.3 TB/s), 16 x 11008 x 4096 11.8 us (3.9 TB/s).
+// distributed shared memory (whole numbers: the order does not matter).  For few tokens, where the weight's bytes, the latency of
+// the first loads and of the join, and uneven shares bind: 1 x 4096 x 11008 10.5 us (4.3 TB/s), 16 x 11008 x 4096 11.8 us (3.9 TB/s).
+// Whole blocks of clusters do not fill the machine: 344 of 128 KB on 132 SMs put 384 KB on the busiest, where an even share of 148
+// is 298 KB, and 256 of 176 KB in clusters of eight on 120 SMs put 528 KB there.
 // DIRECT: operands off the 16-byte grid, brought by warps 2 .. 7 instead of TMA.
 template <typename T, bool KN, bool DIRECT>
 __global__ void __launch_bounds__(I8_THREADS) k_int8_umma(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Operands in,
@@ -583,8 +585,8 @@ inline int blocks_at_once(int split, int room) { return (split <= 2 ? 148 : spli
 // `off_grid`: bytes of the operands that TMA cannot read in place.  They are copied first (4.7 MB a us, read and written, and a
 // launch more: 4 us, most of it the host's), or, where a tile has few slices, shifted on their way: about 4.4 us for a block's first
 // slice and its end and 1.3 us for each other one, 1.7 us with two blocks an SM (fitted to 406 measured plans of 52 shapes, 9 % off;
-// us with / without a copy, without the host's part: 15 x 77 x 1125 5.8 / 4.7, 2 x 1925 x 1098 8.0 / 6.6, 172 x 581 x 516 7.4 / 8.4,
-// 16 x 11007 x 4095 31 / 25, 100 x 4095 x 11007 36 / 64).
+// us with / without a copy, without the host's part, the better plan of each: 15 x 77 x 1125 5.3 / 4.1, 2 x 1925 x 1098 7.7 / 6.2,
+// 172 x 581 x 516 6.5 / 8.0, 16 x 11007 x 4095 30 / 25, 100 x 4095 x 11007 33 / 63).
 Plan make_plan(int m, int k, int n, int64_t off_grid) {
     const int slices = (k + I8_KS - 1) / I8_KS, n128 = (n + 127) / 128, n256 = (n + 255) / 256;
     const float from_hbm = (float)k * n + (float)m * k + 2.0f * m * n, hbm = from_hbm / 5.44e6f, hbm_pairs = from_hbm / 6.26e6f;

@@ -6,7 +6,8 @@
 //
 // Bound by HBM: a row is read once and stays in the registers of its block (up to 128 KB of row), the maximum meets in shared
 // memory, and the row leaves as bytes; a longer row is read twice, the second time from L2.  11008 x 4096 fp32 34 us (6.7 TB/s),
-// bf16 22 us (6.1 TB/s); 1000 x 11008 bf16 7.0 us (4.7 TB/s: one wave of blocks, whose load and store phases hardly overlap).
+// bf16 21.7 us (6.2 TB/s); 1000 x 11008 bf16 7.0 us (4.7 TB/s: 192 threads of 64 registers, so five blocks an SM and 740 of the 1000 at
+// once; the others follow as a short second wave, and load and store phases hardly overlap).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

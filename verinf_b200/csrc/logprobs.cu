@@ -15,7 +15,8 @@
 // of a row, are read again (from L2), what is not below the key is collected and ranked by counting.
 //
 // Bound by HBM where rows are many: 4096 x 32000 bf16 without a list 49 us, 5 us of start and then 6.0 TB/s; the list's instructions
-// come on top.  Few rows are latency: the loads of a thread, the joins of a block and of a cluster.
+// come on top.  Few rows are latency: a thread's rounds of loads (64 x 202045 fp16 in clusters of four: 25 packs a thread in seven
+// rounds with one round ahead, 13.3 us, without a list 10.3), the joins of a block and of a cluster.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
