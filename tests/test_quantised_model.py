@@ -1081,3 +1081,87 @@ def test_matmul_many_tiles_a_pair(i8, layout, m, k, n):
         tol = want.abs() * (3 * HALF[torch.float32] + (HALF[dtype] if dtype != torch.float32 else 0)) * 1.001 + 1e-37
         assert ((y - want).abs() <= tol).all()
     i8.check_async_errors()
+
+
+@gpu
+def test_first_calls_inside_a_capture():
+    """In a process that has called nothing before, the first call of each operator may be a captured one: kernels, their shared memory
+    and tensor maps are set up on the way."""
+    prog = """
+import torch
+from verinf_b200 import int8, logprobs
+x = torch.zeros(300, 512, device="cuda")
+w = torch.zeros(1024, 512, device="cuda")
+a = torch.zeros(40, 515, dtype=torch.int8, device="cuda")
+b = torch.zeros(515, 301, dtype=torch.int8, device="cuda")
+c = torch.zeros(700, 2001, dtype=torch.int8, device="cuda")
+d = torch.zeros(2001, 1500, dtype=torch.int8, device="cuda")
+tokens = torch.zeros(300, dtype=torch.int64, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q, s = int8.int8_quantize_rows(x)
+    wq, ws = int8.int8_quantize_rows(w)
+    logits = int8.int8_matmul(q, wq.t(), s, ws, dtype=torch.float32)
+    one = int8.int8_matmul(q[:1], wq.t())
+    shifted, copied = int8.int8_matmul(a, b), int8.int8_matmul(c, d)
+    out = logprobs.token_logprobs(logits, tokens, top=3)
+for t in (x, w):
+    t.normal_()
+for t in (a, b, c, d):
+    t.random_(-128, 128)
+graph.replay()
+torch.cuda.synchronize()
+sums = lambda p, r: (p.double() @ r.double()).to(torch.int32)
+assert torch.equal(one, sums(q[:1], wq.t())) and torch.equal(shifted, sums(a, b)) and torch.equal(copied, sums(c, d))
+assert torch.equal(logits, sums(q, wq.t()).float() * s[:, None] * ws)
+again = logprobs.token_logprobs(logits, tokens, top=3)
+assert all(torch.equal(p, r) for p, r in zip(out, again))
+assert torch.equal(q, int8.int8_quantize_rows(x)[0]) and int(q.abs().max()) == 127
+int8.check_async_errors()
+print("captured")
+"""
+    root = Path(__file__).resolve().parents[1]
+    out = subprocess.run([sys.executable, "-c", prog], cwd=root, capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0 and out.stdout.strip() == "captured", out.stderr[-2000:]
+
+
+@gpu
+def test_two_threads_at_once(i8, lp):
+    """Calls from two threads, each on a stream of its own, products that are copied and shifted among them, and errors asked for
+    meanwhile."""
+    import threading
+    g = torch.Generator().manual_seed(18)
+    shapes = [[(300, 2001, 1501), (33, 515, 301), (1, 4096, 512)], [(120, 4001, 1003), (333, 1001, 515), (513, 640, 272)]]
+    work = [[(_rand8(g, m, k).cuda(), _rand8(g, k, n).cuda()) for m, k, n in s] for s in shapes]
+    rows = [torch.randn(70, 5003, generator=g).cuda() for _ in range(2)]
+    tokens = torch.arange(70, device="cuda")
+    torch.cuda.synchronize()
+    results, failures = [[], []], []
+
+    def run(j):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(12):
+                    for A, B in work[j]:
+                        results[j].append(i8.int8_matmul(A, B))
+                    results[j].append((i8.int8_quantize_rows(rows[j])[0], lp.token_logprobs(rows[j], tokens, top=7)))
+                    if i % 4 == j:
+                        i8.check_async_errors()
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:
+            failures.append(e)
+
+    threads = [threading.Thread(target=run, args=(j,)) for j in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for j in range(2):
+        sums = [_sums_64(A, B) for A, B in work[j]]
+        q, out = _quantize_64(rows[j])[0], lp.token_logprobs(rows[j], tokens, top=7)
+        for i, y in enumerate(results[j]):
+            if i % 4 < 3:
+                assert torch.equal(y.cpu().long(), sums[i % 4])
+            else:
+                assert torch.equal(y[0].cpu(), q) and all(torch.equal(a, b) for a, b in zip(y[1], out))
